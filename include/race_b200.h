@@ -371,6 +371,82 @@ int race_ace_bwd(const void *Q, const void *K, const void *V, const void *dO, in
                  float eps, float logit_scale,
                  void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- operators around the layer ------------------------------------------------
+ * What a decoder runs next to its RACE layers (no counterpart in the reference,
+ * which takes them from torch: chat/nanochat/gpt.py:51-176): the residual RMS norm,
+ * rows in 8 bits, the 8-bit matrix product, and token log probabilities.
+ *
+ * Tensors are rows of `dtype` values (RACE_F32/RACE_BF16) with unit stride inside a
+ * row.  Inputs may have any row stride (in elements) of at least the row's length;
+ * outputs are dense except 8-bit rows.  All arithmetic is fp32, rounded once into
+ * the output's type.  Two calls may run at the same time on different outputs. */
+
+/* h = x + residual, rounded to dtype;  y = h * rsqrt(mean(h^2) + eps) * weight.
+ * residual may be NULL (h is x; nothing is written to h, which may be NULL).  weight
+ * [K] of weight_dtype may be NULL (ones).  rstd [rows] fp32 (may be NULL) receives
+ * the rows' 1/sqrt(mean(h^2) + eps), which the backward takes. */
+int race_rms_norm_fwd(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, int dtype,
+                      const void *weight, int weight_dtype, void *y, void *h, float *rstd, int64_t rows, int64_t K,
+                      float eps, void *stream);
+
+/* Gradients of race_rms_norm_fwd from dense dy, dh (may be NULL: zero) and h [rows,K]:
+ * dx [rows,K] (the gradient of x and of residual alike) and dw [K] of weight_dtype
+ * (may be NULL: not wanted; then no workspace is needed).  dw is summed in a fixed
+ * order: the same bits every run on the same device. */
+size_t race_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t K);
+int race_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float *rstd, int dtype, const void *weight,
+                      int weight_dtype, void *dx, void *dw, int64_t rows, int64_t K, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
+/* 8-bit rows: q[r, k] = round_to_nearest_even(v[r, k] / scale[r]), scale[r] =
+ * max_k |v[r, k]| / 127 (fp32).  A row of zeros has scale 0 and q = 0; a row holding a
+ * NaN has scale NaN, one holding an infinity scale infinity (so products of it are not
+ * finite).  q_stride (bytes) >= K; race_int8_linear wants it a multiple of 16.
+ *   race_quant_int8:     v = x
+ *   race_rms_norm_int8:  v = the y of race_rms_norm_fwd, not rounded in between; h as there
+ *   race_swiglu_int8:    v = silu(gate) * up of rows [gate F | up F]
+ *   race_dequant_int8:   out[r, k] = q[r, k] * scale[r], rounded to dtype */
+int race_quant_int8(const void *x, int64_t x_stride, int dtype, int8_t *q, int64_t q_stride, float *scale, int64_t rows,
+                    int64_t K, void *stream);
+int race_rms_norm_int8(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, int dtype,
+                       const void *weight, int weight_dtype, int8_t *q, int64_t q_stride, float *scale, void *h,
+                       int64_t rows, int64_t K, float eps, void *stream);
+int race_swiglu_int8(const void *gate_up, int64_t stride, int dtype, int8_t *q, int64_t q_stride, float *scale,
+                     int64_t rows, int64_t F, void *stream);
+int race_dequant_int8(const int8_t *q, int64_t q_stride, const float *scale, void *out, int dtype, int64_t rows,
+                      int64_t K, void *stream);
+
+/* y[m, n] = (sum_k xq[m, k] wq[n, k]) * x_scale[m] * w_scale[n] + bias[n], y dense
+ * [M, N] of dtype; bias [N] fp32 may be NULL.  The integer sum is exact (K <= 131071).
+ * xq, wq and their row strides (bytes) must be multiples of 16 (else RACE_ERR_ALIGN):
+ * the tiles come in by TMA.  Its device-side waits are bounded like the layer's
+ * (race_set_wait_limit); there is no workspace, so a call whose wait gave up writes NaN,
+ * and under race_set_status_check(1) returns RACE_ERR_TIMEOUT. */
+int race_int8_linear(const int8_t *xq, int64_t x_stride, const float *x_scale, const int8_t *wq, int64_t w_stride,
+                     const float *w_scale, const float *bias, void *y, int dtype, int64_t M, int64_t N, int64_t K,
+                     void *stream);
+
+/* Per row of logits [rows, V] (row stride in elements), z = logits / temperature:
+ *   logp = z[token] - log sum exp z;  entropy = -sum p log p (nats)
+ *   top_ids / top_logp [rows, n_top]: the n_top <= min(32, V) largest entries in the
+ *   order (value descending, index ascending) and their log probabilities.
+ * lse [rows, 2] (8-byte aligned) is what the backward takes: the largest logit, and
+ * log2 of the sum of exp(z) relative to its own.  Entries of -infinity have probability 0; a row
+ * of them alone has logp -infinity and entropy 0.  A NaN or +infinity in a row makes its logp and entropy NaN
+ * (a NaN ranks as -infinity among the alternatives).  A row whose token is ignore_index
+ * has logp and entropy 0, ids -1 and top_logp -infinity; any other token outside
+ * [0, V) has logp NaN. */
+int race_token_logprobs_fwd(const void *logits, int64_t stride, int dtype, const int64_t *tokens, int64_t ignore_index,
+                            float temperature, int n_top, float *logp, float *entropy, float *lse, int64_t *top_ids,
+                            float *top_logp, int64_t rows, int64_t V, void *stream);
+
+/* dlogits [rows, V] dense, of dtype, for the gradients g_logp and g_entropy [rows] fp32
+ * (either may be NULL: zero) of logp and entropy, from the forward's lse and entropy.
+ * Ignored rows, and rows of -infinity alone, get 0. */
+int race_token_logprobs_bwd(const void *logits, int64_t stride, int dtype, const int64_t *tokens, int64_t ignore_index,
+                            float temperature, const float *lse, const float *entropy, const float *g_logp,
+                            const float *g_entropy, void *dlogits, int64_t rows, int64_t V, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -74,9 +74,20 @@ SIGNATURES = {
                           _SZ, _P],
     "race_bwd_qkv_saved": [_P, _P, _P, _P, _I, _P, _P, _SZ, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                            _I64, _I64, _I64, _I64, _I64, _F, _F, _P, _SZ, _P],
+    "race_rms_norm_fwd": [_P, _I64, _P, _I64, _I, _P, _I, _P, _P, _P, _I64, _I64, _F, _P],
+    "race_rms_norm_bwd_workspace_bytes": [_I64, _I64],
+    "race_rms_norm_bwd": [_P, _P, _P, _P, _I, _P, _I, _P, _P, _I64, _I64, _P, _SZ, _P],
+    "race_quant_int8": [_P, _I64, _I, _P, _I64, _P, _I64, _I64, _P],
+    "race_rms_norm_int8": [_P, _I64, _P, _I64, _I, _P, _I, _P, _I64, _P, _P, _I64, _I64, _F, _P],
+    "race_swiglu_int8": [_P, _I64, _I, _P, _I64, _P, _I64, _I64, _P],
+    "race_dequant_int8": [_P, _I64, _P, _P, _I, _I64, _I64, _P],
+    "race_int8_linear": [_P, _I64, _P, _P, _I64, _P, _P, _P, _I, _I64, _I64, _I64, _P],
+    "race_token_logprobs_fwd": [_P, _I64, _I, _P, _I64, _F, _I, _P, _P, _P, _P, _P, _I64, _I64, _P],
+    "race_token_logprobs_bwd": [_P, _I64, _I, _P, _I64, _F, _P, _P, _P, _P, _P, _I64, _I64, _P],
 }
 _RESTYPES = {"race_status_string": ctypes.c_char_p, "race_last_error": ctypes.c_char_p,
-             "race_launch_counter": ctypes.c_ulonglong, "race_gqa_decode_workspace_bytes": ctypes.c_size_t}
+             "race_launch_counter": ctypes.c_ulonglong, "race_gqa_decode_workspace_bytes": ctypes.c_size_t,
+             "race_rms_norm_bwd_workspace_bytes": ctypes.c_size_t}
 
 
 def library_path() -> str:

@@ -762,6 +762,23 @@ int report_error(int code, const char *msg) {
 }
 void clear_error() { g_err[0] = 0; }
 void note_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+
+uint32_t current_wait_limit() { return wait_limit(); }
+bool status_check_on() { return g_status_check.load(std::memory_order_relaxed) != 0; }
+bool withhold_first_load() { return g_withhold_first_load.load(std::memory_order_relaxed) != 0; }
+
+bool make_byte_rows_map(void *map, const void *base, int64_t rows, int64_t cols, int64_t row_stride, int box_rows) {
+  if (!fasthost::bind_current_context()) return false;
+  fasthost::EncodeTiledFn enc = fasthost::encoder();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)row_stride};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  cuuint32_t es[2] = {1, 1};
+  return enc(reinterpret_cast<CUtensorMap *>(map), CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims,
+             strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 }  // namespace race
 
 // ============================================================================

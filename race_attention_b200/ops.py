@@ -508,3 +508,237 @@ def gqa_decode_attention(q, k_new, v_new, k_cache, v_cache, length, workspace, n
                                             _ptr(length), _ptr(out), _ptr(workspace), B, Hq, Hkv, Tmax, D,
                                             int(n_splits), scale, _stream(dev)), "race_gqa_decode_attn")
     return out
+
+
+# ---------------------------------------------------------------------------
+# operators around the layer: residual RMS norm, 8-bit rows and products, token log
+# probabilities.  Some of them run for a few microseconds on a decode step, so they
+# launch without entering a device context where the tensors' device is current.
+def _launch(dev, name, *args):
+    """Call C entry point `name` with args and the current stream of `dev`."""
+    fn = getattr(_lib.load(), name)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _rows(x, name):
+    """x [..., K] as (rows with unit stride inside a row, row stride, rows, K): a view where
+    the rows are evenly spaced, else a copy."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"{name} must have rows of at least one value")
+    K = x.shape[-1]
+    if x.is_contiguous():
+        return x, K, x.numel() // K, K
+    if x.dim() != 2:
+        x = x.reshape(-1, K)
+    rows, stride = x.shape[0], x.stride(0)
+    if x.stride(1) != 1 or (stride < K and rows > 1):  # strided or overlapping (expanded) rows
+        x, stride = x.contiguous(), K
+    return x, max(stride, K), rows, K
+
+
+def _weight_code(weight, K):
+    if weight is None:
+        return _lib.RACE_F32
+    if weight.shape != (K,) or not weight.is_contiguous():
+        raise RuntimeError(f"weight must be a contiguous [{K}] tensor")
+    return _dtype_code(weight)
+
+
+def _norm_inputs(x, residual, weight):
+    dev = _check_cuda(x, residual, weight)
+    code = _dtype_code(x)
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise RuntimeError("residual must have x's shape and dtype")
+    xr, xs, rows, K = _rows(x, "x")
+    rr, rs = (None, 0) if residual is None else _rows(residual, "residual")[:2]
+    return dev, code, xr, xs, rr, rs, rows, K, _weight_code(weight, K)
+
+
+def _ptr_of(t):
+    return None if t is None else t.data_ptr()
+
+
+def rms_norm_fwd(x, residual=None, weight=None, eps=1e-5, return_rstd=False):
+    """(y, h[, rstd]): h = x + residual in x's dtype (x itself without a residual),
+    y = h * rsqrt(mean(h^2) + eps) * weight; x [..., K]."""
+    dev, code, xr, xs, rr, rs, rows, K, wc = _norm_inputs(x, residual, weight)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if return_rstd else None
+    if rows:
+        _launch(dev, "race_rms_norm_fwd", xr.data_ptr(), xs, _ptr_of(rr), rs, code, _ptr_of(weight), wc, y.data_ptr(),
+                None if residual is None else h.data_ptr(), _ptr_of(rstd), rows, K, eps)
+    return (y, h, rstd) if return_rstd else (y, h)
+
+
+def rms_norm_bwd(dy, dh, h, rstd, weight=None, weight_grad=True):
+    """(dx, dw) of rms_norm_fwd for the gradients dy of y and dh of h (None: zero); dx is the
+    gradient of x and of the residual alike, dw (None unless weight_grad) has weight's dtype."""
+    dev = _check_cuda(dy, dh, h, rstd, weight)
+    code = _dtype_code(h)
+    K = h.shape[-1]
+    if dy.shape != h.shape or dy.dtype != h.dtype or (dh is not None and (dh.shape != h.shape or dh.dtype != h.dtype)):
+        raise RuntimeError("dy and dh must have h's shape and dtype")
+    rows = h.numel() // K
+    if rstd.dtype != torch.float32 or rstd.numel() != rows:
+        raise RuntimeError(f"rstd must hold {rows} float32 values")
+    wc = _weight_code(weight, K)
+    dy, h, rstd = dy.contiguous(), h.contiguous(), rstd.contiguous()
+    dh = None if dh is None else dh.contiguous()
+    dx = torch.empty(h.shape, dtype=h.dtype, device=dev)
+    dw = ws = None
+    nb = 0
+    if weight_grad:
+        dw = torch.empty(K, dtype=torch.float32 if weight is None else weight.dtype, device=dev)
+        nb = int(_lib.load().race_rms_norm_bwd_workspace_bytes(rows, K)) if rows else 0
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    if rows:
+        _launch(dev, "race_rms_norm_bwd", dy.data_ptr(), _ptr_of(dh), h.data_ptr(), rstd.data_ptr(), code,
+                _ptr_of(weight), wc, dx.data_ptr(), _ptr_of(dw), rows, K, _ptr_of(ws), nb)
+    elif dw is not None:
+        dw.zero_()
+    return dx, dw
+
+
+def _int8_out(shape, dev):
+    """8-bit rows [..., K] whose rows start at multiples of 16 bytes (what the 8-bit product's
+    tile loads need), their row stride, and their scales [...]."""
+    K = shape[-1]
+    rows = math.prod(shape[:-1])
+    stride = -(-K // 16) * 16
+    q = torch.empty((rows, stride), dtype=torch.int8, device=dev)
+    if stride != K:
+        q = q[:, :K]
+    if len(shape) != 2:
+        q = q.unflatten(0, shape[:-1]) if len(shape) > 2 else q[0]
+    return q, stride, torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+
+
+def rms_norm_int8(x, residual=None, weight=None, eps=1e-5):
+    """(q, scale, h): the y of rms_norm_fwd as 8-bit rows (not rounded in between), and h."""
+    dev, code, xr, xs, rr, rs, rows, K, wc = _norm_inputs(x, residual, weight)
+    q, qs, scale = _int8_out(x.shape, dev)
+    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if rows:
+        _launch(dev, "race_rms_norm_int8", xr.data_ptr(), xs, _ptr_of(rr), rs, code, _ptr_of(weight), wc, q.data_ptr(),
+                qs, scale.data_ptr(), None if residual is None else h.data_ptr(), rows, K, eps)
+    return q, scale, h
+
+
+def quant_int8(x):
+    """(q, scale): x [..., K] as 8-bit rows."""
+    dev = _check_cuda(x)
+    code = _dtype_code(x)
+    xr, xs, rows, K = _rows(x, "x")
+    q, qs, scale = _int8_out(x.shape, dev)
+    if rows:
+        _launch(dev, "race_quant_int8", xr.data_ptr(), xs, code, q.data_ptr(), qs, scale.data_ptr(), rows, K)
+    return q, scale
+
+
+def swiglu_int8(gate_up):
+    """(q, scale): silu(gate) * up of gate_up [..., 2 F] = [gate | up] as 8-bit rows [..., F]."""
+    dev = _check_cuda(gate_up)
+    code = _dtype_code(gate_up)
+    xr, xs, rows, K2 = _rows(gate_up, "gate_up")
+    if K2 % 2:
+        raise RuntimeError("gate_up must hold an even number of values per row")
+    q, qs, scale = _int8_out(gate_up.shape[:-1] + (K2 // 2,), dev)
+    if rows:
+        _launch(dev, "race_swiglu_int8", xr.data_ptr(), xs, code, q.data_ptr(), qs, scale.data_ptr(), rows, K2 // 2)
+    return q, scale
+
+
+def _int8_rows(q, scale, name):
+    if q.dtype != torch.int8 or scale.dtype != torch.float32 or scale.shape != q.shape[:-1]:
+        raise RuntimeError(f"{name} must be int8 rows [..., K] with float32 scales [...]")
+    return *_rows(q, name), scale.contiguous()
+
+
+def dequant_int8(q, scale, dtype=torch.bfloat16):
+    """q * scale, rounded to dtype."""
+    dev = _check_cuda(q, scale)
+    qr, qs, rows, K, scale = _int8_rows(q, scale, "q")
+    out = torch.empty(q.shape, dtype=dtype, device=dev)
+    if rows:
+        _launch(dev, "race_dequant_int8", qr.data_ptr(), qs, scale.data_ptr(), out.data_ptr(), _dtype_code(out), rows, K)
+    return out
+
+
+def _aligned_rows(q, stride):
+    """8-bit rows whose starts are multiples of 16 bytes: q, or a padded copy of it."""
+    if stride % 16 == 0 and q.data_ptr() % 16 == 0:
+        return q, stride
+    K = q.shape[-1]
+    stride = -(-K // 16) * 16
+    p = torch.empty((q.numel() // K, stride), dtype=torch.int8, device=q.device)[:, :K]
+    p.copy_(q.reshape(-1, K))
+    return p, stride
+
+
+def int8_linear(xq, x_scale, wq, w_scale, bias=None, dtype=torch.bfloat16):
+    """(xq . wq^T) * x_scale * w_scale + bias: xq int8 [..., K], wq int8 [N, K], scales and bias
+    float32 -> [..., N] of dtype.  Rows that start at multiples of 16 bytes (as the quantisers
+    here lay them out) are read in place; others are copied first."""
+    dev = _check_cuda(xq, x_scale, wq, w_scale, bias)
+    xr, xs, M, K, x_scale = _int8_rows(xq, x_scale, "x")
+    if wq.dim() != 2 or wq.shape[1] != K:
+        raise RuntimeError(f"w must be int8 [N, {K}]")
+    wr, ws, N, _, w_scale = _int8_rows(wq, w_scale, "w")
+    if bias is not None and (bias.shape != (N,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
+        raise RuntimeError(f"bias must be a contiguous float32 [{N}] tensor")
+    y = torch.empty(xq.shape[:-1] + (N,), dtype=dtype, device=dev)
+    code = _dtype_code(y)
+    if M and N:
+        xr, xs = _aligned_rows(xr, xs)
+        wr, ws = _aligned_rows(wr, ws)
+        _launch(dev, "race_int8_linear", xr.data_ptr(), xs, x_scale.data_ptr(), wr.data_ptr(), ws, w_scale.data_ptr(),
+                _ptr_of(bias), y.data_ptr(), code, M, N, K)
+    return y
+
+
+def _logit_rows(logits, tokens):
+    dev = _check_cuda(logits, tokens)
+    if tokens.dtype != torch.int64 or tokens.shape != logits.shape[:-1]:
+        raise RuntimeError("tokens must be int64 of the logits' shape without its last dimension")
+    return dev, _dtype_code(logits), *_rows(logits, "logits"), tokens.contiguous()
+
+
+def token_logprobs_fwd(logits, tokens, temperature=1.0, n_top=0, ignore_index=-100):
+    """(logp, entropy, lse, top_ids, top_logp) of logits [..., V] at tokens [...]; the last two are
+    [..., n_top], lse [..., 2] is for the backward.  See race_token_logprobs_fwd in include/race_b200.h for masked and ignored rows."""
+    dev, code, lr, ls, rows, V, tokens = _logit_rows(logits, tokens)
+    n_top = int(n_top)
+    shape = tokens.shape
+    logp = torch.empty(shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(shape, dtype=torch.float32, device=dev)
+    lse = torch.empty(shape + (2,), dtype=torch.float32, device=dev)
+    top_ids = torch.empty(shape + (max(n_top, 0),), dtype=torch.int64, device=dev)
+    top_logp = torch.empty(shape + (max(n_top, 0),), dtype=torch.float32, device=dev)
+    if rows:
+        _launch(dev, "race_token_logprobs_fwd", lr.data_ptr(), ls, code, tokens.data_ptr(), int(ignore_index),
+                float(temperature), n_top, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top_ids.data_ptr(),
+                top_logp.data_ptr(), rows, V)
+    return logp, entropy, lse, top_ids, top_logp
+
+
+def token_logprobs_bwd(logits, tokens, lse, entropy, g_logp, g_entropy, temperature=1.0, ignore_index=-100):
+    """dlogits of token_logprobs_fwd for the gradients g_logp, g_entropy (None: zero)."""
+    dev, code, lr, ls, rows, V, tokens = _logit_rows(logits, tokens)
+    _check_cuda(logits, lse, entropy, g_logp, g_entropy)
+    lse, entropy, g_logp, g_entropy = (None if t is None else t.float().contiguous()
+                                       for t in (lse, entropy, g_logp, g_entropy))
+    if lse.numel() != 2 * rows or any(t is not None and t.numel() != rows for t in (entropy, g_logp, g_entropy)):
+        raise RuntimeError(f"lse must hold {2 * rows} values, entropy and the gradients {rows}")
+    d = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    if rows:
+        _launch(dev, "race_token_logprobs_bwd", lr.data_ptr(), ls, code, tokens.data_ptr(), int(ignore_index),
+                float(temperature), lse.data_ptr(), entropy.data_ptr(), _ptr_of(g_logp), _ptr_of(g_entropy),
+                d.data_ptr(), rows, V)
+    return d
