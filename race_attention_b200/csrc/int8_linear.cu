@@ -2,13 +2,23 @@
 // and per output channel) on the tcgen05 integer tensor cores.
 //
 // Mathematics: y[m, n] = (sum_k xq[m, k] wq[n, k]) * xs[m] * ws[n] + bias[n].  The sum is
-// an exact 32-bit integer (widths up to 131071 cannot overflow it, even at -128 * -128);
-// it is scaled in fp32 and rounded once to the output's type.
+// an exact 32-bit integer (widths up to 131071 cannot overflow it, even at -128 * -128), in
+// whatever order its parts are added; it is scaled in fp32 and rounded once to the output's
+// type.
 //
-// One CTA computes a 128 x 128 tile: a producer lane streams 128-byte-wide K slices of
-// both operands through a ring of shared-memory stages by TMA (rows and bytes past the
-// tensors' ends read as 0, so ragged sizes need no special case), a second lane issues
-// tcgen05.mma kind::i8 into a TMEM accumulator, and four warps scale and store it.
+// Operands come in as 128-byte-wide K slices by TMA (128-byte swizzle), through a ring of
+// shared-memory stages; rows and bytes past the tensors' ends read as 0, so ragged sizes need
+// no special case.  One lane issues the copies, one the tcgen05.mma kind::i8, and four warps
+// scale and store the accumulators they read from TMEM.  Two kernels share that scheme:
+//
+// * split_kernel, for few tokens: the weights are the MMA's rows (128 channels per CTA), the
+//   tokens its columns (16 to 128), so a weight byte is read once and the tensor cores idle
+//   under a stream of weights.  Up to 8 CTAs of a cluster share a tile's K range and add their
+//   integer sums through each other's shared memory, which gives every SM weights to stream
+//   when the layer has few channels, with no workspace and no atomics.
+// * pair_kernel, for many: a pair of CTAs computes 256 tokens x 256 channels with
+//   cta_group::2 (each SM holds half of either operand), persistent over the tiles, with two
+//   accumulators in TMEM so that one tile's stores overlap the next one's products.
 #include "race_b200.h"
 
 #include <math.h>
@@ -25,13 +35,13 @@ namespace tc = race::tc;
 using race::cuda_err;
 using race::err;
 
-constexpr int kBM = 128, kBN = 128, kBK = 128;  // tile rows, channels, K bytes per stage
-constexpr int kStages = 6;
-constexpr int kThreads = 192;  // producer warp, MMA warp, four epilogue warps
-constexpr int kABytes = kBM * kBK, kBBytes = kBN * kBK;
-constexpr int kSmem = kStages * (kABytes + kBBytes) + 1024;
+constexpr int kBK = 128;                  // K bytes per stage (one swizzled row)
+constexpr int kTileRows = 128;            // operand rows per tile and CTA
+constexpr int kTileBytes = kTileRows * kBK;
+constexpr int kThreads = 192;             // producer warp, MMA warp, four epilogue warps
 constexpr int kMaxDevices = 128;
-constexpr int64_t kMaxK = 131071;  // 2^31 / 128^2, less one
+constexpr int64_t kMaxK = 131071;         // 2^31 / 128^2, less one
+constexpr int kMaxSplit = 8;              // CTAs of a cluster that share a tile's K range
 
 // Set by a kernel whose bounded wait gave up (its outputs are NaN); read and cleared by
 // calls made under race_set_status_check(1).
@@ -40,8 +50,10 @@ __device__ int g_timeout;
 struct Args {
   const float *xs, *ws, *bias;
   void *y;
-  long long M, N;
-  int k_steps, vec_ok, withhold;
+  int M, N, k_steps;
+  int m_tiles, n_tiles;  // pair_kernel
+  int vec_ok;            // output rows start at multiples of 16 bytes
+  int withhold;
   uint32_t wait_limit;
 };
 
@@ -50,106 +62,452 @@ constexpr uint32_t idesc_i8(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
+template <int CG>
 __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_constant__ CUtensorMap mx,
-                                                             const __grid_constant__ CUtensorMap mw, const Args a) {
+// One stage's products: 128 bytes of K in steps of 32.
+template <int CG>
+__device__ __forceinline__ void mma_stage(uint32_t d_tmem, uint32_t sa, uint32_t sb, uint32_t idesc, bool first) {
+#pragma unroll
+  for (int j = 0; j < kBK / 32; ++j)
+    mma_i8<CG>(d_tmem, tc::sdesc(sa + 32 * j, 16, 1024), tc::sdesc(sb + 32 * j, 16, 1024), idesc, !(first && j == 0));
+}
+
+// ---- cluster helpers
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t smem_addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
+  return r;
+}
+// every thread of every CTA of the cluster
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ int4 ld_cluster_i4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ int ld_cluster_i(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// ---- a pair of CTAs (cta_group::2)
+// Tile load into this CTA's shared memory that completes on the pair leader's barrier.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, uint32_t leader_bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(leader_bar)
+      : "memory");
+}
+// One arrival on the barrier at this offset in both CTAs once the MMAs issued so far are done.
+__device__ __forceinline__ void commit_pair(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(tc::smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t *dst, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(dst)), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t addr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(ncols) : "memory");
+}
+
+__device__ __forceinline__ unsigned char *align_1k(unsigned char *p) {
+  return reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
+}
+
+// ------------------------------------------------------------------ few tokens
+template <int BT>
+struct Split {
+  static constexpr int kStageBytes = kTileBytes + BT * kBK;
+  // about 96 KB in flight per CTA, two CTAs per SM
+  static constexpr int kStages = BT <= 16 ? 5 : BT <= 32 ? 5 : BT <= 64 ? 4 : 3;
+  static constexpr int kSum = BT * kTileRows * 4;  // one CTA's integer sums, over the ring's stages
+  static constexpr int kBytes = (kStages * kStageBytes > kSum ? kStages * kStageBytes : kSum) + 1024;
+  static constexpr int kCols = BT < 32 ? 32 : BT;  // TMEM columns (a power of two of at least 32)
+};
+
+// Grid (S * channel tiles, token tiles), clusters of S along x: rank r of a cluster takes the
+// r-th S-th of the K steps, then sums and stores channels [r, r + 1) * 128 / S of the tile.
+template <typename T, int BT>
+__global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__ CUtensorMap mx,
+                                                         const __grid_constant__ CUtensorMap mw, const Args a, const int S) {
+  using C = Split<BT>;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t full[kStages], empty[kStages], done;
+  __shared__ uint64_t full[C::kStages], empty[C::kStages], done;
   __shared__ uint32_t tmem_slot;
   __shared__ int ctl[2];  // {abort flag, poll limit}
-  unsigned char *ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char *ring = align_1k(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long m0 = (long long)blockIdx.y * kBM, n0 = (long long)blockIdx.x * kBN;
+  const int rank = blockIdx.x % S, n0 = (int)(blockIdx.x / S) * kTileRows, m0 = blockIdx.y * BT;
+  const int k_begin = (int)((long long)a.k_steps * rank / S), k_end = (int)((long long)a.k_steps * (rank + 1) / S);
+  const int steps = k_end - k_begin;
   volatile int *abort = ctl;
 
   if (threadIdx.x == 0) {
+    tc::prefetch_tmap(&mx);
+    tc::prefetch_tmap(&mw);
     ctl[0] = 0;
     ctl[1] = (int)a.wait_limit;
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < C::kStages; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
     }
     tc::mbar_init(&done, 1);
     tc::fence_mbar_init();
   }
-  if (warp == 1) tc::tmem_alloc(&tmem_slot, kBN);
+  if (warp == 1) tc::tmem_alloc(&tmem_slot, C::kCols);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp == 0 && lane == 0) {
-    int issued = 0;
-    for (int k = 0; k < (a.withhold ? 0 : a.k_steps); ++k) {
-      const int st = k % kStages, use = k / kStages;
-      if (use && !tc::mbar_wait(&empty[st], (use - 1) & 1, abort)) break;
-      unsigned char *sa = ring + st * (kABytes + kBBytes);
-      tc::mbar_arrive_expect_tx(&full[st], kABytes + kBBytes);
-      tc::tma_load_2d(sa, &mx, &full[st], k * kBK, (int)m0);
-      tc::tma_load_2d(sa + kABytes, &mw, &full[st], k * kBK, (int)n0);
-      issued = k + 1;
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = 0;
+      for (int k = 0; k < (a.withhold ? 0 : steps); ++k) {
+        const int st = k % C::kStages, use = k / C::kStages;
+        if (use && !tc::mbar_wait(&empty[st], (use - 1) & 1, abort)) break;
+        unsigned char *sw = ring + st * C::kStageBytes;
+        tc::mbar_arrive_expect_tx(&full[st], C::kStageBytes);
+        tc::tma_load_2d(sw, &mw, &full[st], (k_begin + k) * kBK, n0);
+        tc::tma_load_2d(sw + kTileBytes, &mx, &full[st], (k_begin + k) * kBK, m0);
+        issued = k + 1;
+      }
+      if (*abort)  // no copy may land after the block has gone
+        for (int k = issued > C::kStages ? issued - C::kStages : 0; k < issued; ++k)
+          tc::mbar_wait_drain(&full[k % C::kStages], (k / C::kStages) & 1);
     }
-    if (*abort)  // no copy may land after the block has gone
-      for (int k = issued > kStages ? issued - kStages : 0; k < issued; ++k)
-        tc::mbar_wait_drain(&full[k % kStages], (k / kStages) & 1);
-  } else if (warp == 1 && lane == 0) {
-    constexpr uint32_t id = idesc_i8(kBM, kBN);
-    for (int k = 0; k < a.k_steps; ++k) {
-      const int st = k % kStages;
-      if (!tc::mbar_wait(&full[st], (k / kStages) & 1, abort)) break;
-      tc::tc_fence_after();
-      const uint32_t sa = tc::smem_u32(ring + st * (kABytes + kBBytes)), sb = sa + kABytes;
-#pragma unroll
-      for (int j = 0; j < kBK / 32; ++j)  // 32 bytes of K per instruction
-        mma_i8(tmem, tc::sdesc(sa + 32 * j, 16, 1024), tc::sdesc(sb + 32 * j, 16, 1024), id, k | j);
-      tc::mma_commit(&empty[st]);
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t id = idesc_i8(kTileRows, BT);
+      for (int k = 0; k < steps; ++k) {
+        const int st = k % C::kStages;
+        if (!tc::mbar_wait(&full[st], (k / C::kStages) & 1, abort)) break;
+        tc::tc_fence_after();
+        const uint32_t sw = tc::smem_u32(ring + st * C::kStageBytes);
+        mma_stage<1>(tmem, sw, sw + kTileBytes, id, k == 0);
+        tc::mma_commit(&empty[st]);
+      }
+      tc::mma_commit(&done);
+      if (*abort) tc::mbar_wait_drain(&done, 0);
     }
-    tc::mma_commit(&done);
-    if (*abort) tc::mbar_wait_drain(&done, 0);
-  } else if (warp >= 2) {
+    __syncwarp();
+  } else {
+    // this CTA's sums as [token][channel] integers, over the ring (all its copies are consumed)
     const int quarter = warp & 3;  // the TMEM lanes a warp may read
-    const long long m = m0 + quarter * 32 + lane;
     const bool ok = tc::warp_all(tc::mbar_wait(&done, 0, abort) && !*abort);
     tc::tc_fence_after();
-    const float xs = m < a.M ? a.xs[m] : 0.f;
-    T *y = static_cast<T *>(a.y) + m * a.N;
-    for (int c = 0; c < kBN; c += 32) {
-      float v[32];
-      tc::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
-      tc::tmem_wait_ld();
-      if (m < a.M) {
+    int *sum = reinterpret_cast<int *>(ring) + quarter * 32 + lane;
+    const bool live = ok && steps > 0;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const long long n = n0 + c + j;
-          if (n < a.N) {
-            float f = (float)__float_as_int(v[j]) * xs * __ldg(a.ws + n);
-            if (a.bias) f += __ldg(a.bias + n);
-            y[n] = race::from_f<T>(ok ? f : NAN);
-          }
-        }
+    for (int c = 0; c < BT; c += 16) {
+      float v[16];
+      tc::tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
+      tc::tmem_wait_ld();
+      if (ok) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[(c + j) * kTileRows] = live ? __float_as_int(v[j]) : 0;
       }
-      __syncwarp();  // TMEM loads are whole-warp instructions
+      __syncwarp();
     }
-    if (!ok && lane == 0) atomicExch(&g_timeout, 1);
     tc::tc_fence_before();
   }
-  __syncthreads();
+  cluster_sync();
+
+  // add the cluster's sums for this CTA's channels, scale and store
+  bool ok = true;
+  for (int r = 0; r < S; ++r) ok = ok && ld_cluster_i(map_rank(tc::smem_u32(&ctl[0]), r)) == 0;
+  const int width = kTileRows / S, c0 = rank * width;  // channels of this CTA: 16 to 128
+  const int quads = width / 4;
+  const uint32_t base = tc::smem_u32(ring) + 4 * c0;
+  for (int e = threadIdx.x; e < BT * quads; e += kThreads) {
+    const int t = e / quads, c = 4 * (e % quads);
+    const int m = m0 + t, n = n0 + c0 + c;
+    if (m >= a.M || n >= a.N) continue;
+    int4 acc = make_int4(0, 0, 0, 0);
+    const uint32_t at = base + 4 * (t * kTileRows + c);
+#pragma unroll
+    for (int r = 0; r < kMaxSplit; ++r)
+      if (r < S) {
+        const int4 v = ld_cluster_i4(map_rank(at, r));
+        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+      }
+    const float xs = __ldg(a.xs + m);
+    const int q[4] = {acc.x, acc.y, acc.z, acc.w};
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int nn = min(n + j, a.N - 1);
+      f[j] = (float)q[j] * xs * __ldg(a.ws + nn);
+      if (a.bias) f[j] += __ldg(a.bias + nn);
+      if (!ok) f[j] = NAN;
+    }
+    T *y = static_cast<T *>(a.y) + (long long)m * a.N + n;
+    if (a.vec_ok) {  // N is a multiple of 16 bytes' worth of values: n + 3 < N too
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2 *>(y) = make_uint2(tc::pack_bf16(f[0], f[1]), tc::pack_bf16(f[2], f[3]));
+      else
+        *reinterpret_cast<float4 *>(y) = make_float4(f[0], f[1], f[2], f[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < a.N) y[j] = race::from_f<T>(f[j]);
+    }
+  }
+  if (!ok && threadIdx.x == 0) atomicExch(&g_timeout, 1);
+  cluster_sync();  // nobody leaves while its sums are read
   if (warp == 1) {
-    __syncwarp();
     tc::tc_fence_after();
-    tc::tmem_dealloc(tmem, kBN);
+    tc::tmem_dealloc(tmem, C::kCols);
   }
 }
 
+// ------------------------------------------------------------------ many tokens
+constexpr int kPairStages = 6;
+constexpr int kPairStageBytes = 2 * kTileBytes;
+constexpr int kPairN = 256;               // channels per tile and accumulator columns
+constexpr int kStageOut = 4 * 32 * 128;   // per epilogue warp: 32 rows x 128 bytes on their way out
+constexpr int kPairSmem = kPairStages * kPairStageBytes + kStageOut + 1024;
+constexpr int kGroupM = 8;                // token tiles that share their weight tiles in L2
+
+// The t-th tile: groups of kGroupM token tiles, inside a group the token tile varies fastest.
+__device__ __forceinline__ void tile_at(const Args &a, int t, int &mt, int &nt) {
+  const int group = t / (kGroupM * a.n_tiles);
+  const int in = t - group * (kGroupM * a.n_tiles);
+  const int gm = min(kGroupM, a.m_tiles - group * kGroupM);
+  nt = in / gm;
+  mt = group * kGroupM + in - nt * gm;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) __cluster_dims__(2, 1, 1)
+pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const Args a) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int ctl[2];  // {abort flag, poll limit}
+  __shared__ __align__(16) float scale[kPairN], bias[kPairN];
+  unsigned char *ring = align_1k(smem_raw);
+  unsigned char *out_stage = ring + kPairStages * kPairStageBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles = a.m_tiles * a.n_tiles;
+  volatile int *abort = ctl;
+
+  if (threadIdx.x == 0) {
+    tc::prefetch_tmap(&mx);
+    tc::prefetch_tmap(&mw);
+    ctl[0] = 0;
+    ctl[1] = (int)a.wait_limit;
+    for (int i = 0; i < kPairStages; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&acc_full[i], 1);
+      tc::mbar_init(&acc_empty[i], 8);  // the pair's epilogue warps
+    }
+    tc::mbar_init(&drained, 1);
+    tc::fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc_pair(&tmem_slot, 2 * kPairN);
+  tc::tc_fence_before();
+  cluster_sync();  // both CTAs' barriers exist
+  tc::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0 && !a.withhold) {
+      long long step = 0;  // stages filled so far, over all tiles
+      bool go = true;
+      for (int t = pair; go && t < tiles; t += pairs) {
+        int mt, nt;
+        tile_at(a, t, mt, nt);
+        const int m = mt * 256 + rank * kTileRows, n = nt * kPairN + rank * kTileRows;
+        for (int k = 0; k < a.k_steps; ++k, ++step) {
+          const int st = (int)(step % kPairStages);
+          const long long use = step / kPairStages;
+          if (use && !tc::mbar_wait(&empty[st], (uint32_t)(use - 1) & 1, abort)) {
+            go = false;
+            break;
+          }
+          const uint32_t sa = tc::smem_u32(ring + st * kPairStageBytes);
+          const uint32_t bar = map_rank(tc::smem_u32(&full[st]), 0);
+          // the leader's barrier counts both CTAs' bytes; the peer's may land first
+          if (rank == 0) tc::mbar_arrive_expect_tx(&full[st], 2 * kPairStageBytes);
+          tma_load_pair(sa, &mx, bar, k * kBK, m);
+          tma_load_pair(sa + kTileBytes, &mw, bar, k * kBK, n);
+        }
+      }
+      if (*abort && rank == 0) {  // both CTAs' copies must have landed before either leaves
+        const long long first = step > kPairStages ? step - kPairStages : 0;
+        for (long long s = first; s < step; ++s)
+          tc::mbar_wait_drain(&full[s % kPairStages], (uint32_t)(s / kPairStages) & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t id = idesc_i8(256, kPairN);
+      long long step = 0;
+      int i = 0;
+      bool go = true;
+      for (int t = pair; go && t < tiles; t += pairs, ++i) {
+        const int buf = i & 1, use = i >> 1;
+        if (use && !tc::mbar_wait(&acc_empty[buf], (use - 1) & 1, abort)) break;
+        tc::tc_fence_after();
+        for (int k = 0; k < a.k_steps; ++k, ++step) {
+          const int st = (int)(step % kPairStages);
+          if (!tc::mbar_wait(&full[st], (uint32_t)(step / kPairStages) & 1, abort)) {
+            go = false;
+            break;
+          }
+          tc::tc_fence_after();
+          const uint32_t sa = tc::smem_u32(ring + st * kPairStageBytes);
+          mma_stage<2>(tmem + buf * kPairN, sa, sa + kTileBytes, id, k == 0);
+          commit_pair(&empty[st]);
+        }
+        if (go) commit_pair(&acc_full[buf]);
+      }
+      if (*abort) {
+        commit_pair(&drained);
+        tc::mbar_wait_drain(&drained, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3;
+    const int et = threadIdx.x - 64;  // 0..127 over the epilogue warps
+    const uint32_t stage = tc::smem_u32(out_stage) + quarter * (32 * 128);
+    constexpr int kCols = 128 / (int)sizeof(T);  // columns per 128-byte output row
+    int i = 0;
+    for (int t = pair; t < tiles; t += pairs, ++i) {
+      int mt, nt;
+      tile_at(a, t, mt, nt);
+      const int buf = i & 1, use = i >> 1;
+      const int m0 = mt * 256 + rank * kTileRows + quarter * 32, n0 = nt * kPairN;
+      tc::named_bar_sync(1, 128);  // the last tile's scales are read
+      for (int c = et; c < kPairN; c += 128) {
+        const int n = min(n0 + c, a.N - 1);
+        scale[c] = __ldg(a.ws + n);
+        bias[c] = a.bias ? __ldg(a.bias + n) : 0.f;
+      }
+      const int m = m0 + lane;
+      const float xs = m < a.M ? __ldg(a.xs + m) : 0.f;
+      tc::named_bar_sync(1, 128);
+      const bool ok = tc::warp_all(!*abort && tc::mbar_wait(&acc_full[buf], use & 1, abort));
+      tc::tc_fence_after();
+      const int rows = min(32, a.M - m0);
+#pragma unroll 1
+      for (int c = 0; c < kPairN; c += kCols) {
+        // a row of 128 output bytes per lane, its 16-byte chunks swizzled by the row
+#pragma unroll
+        for (int h = 0; h < kCols; h += 32) {
+          float v[32];
+          tc::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + buf * kPairN + c + h, v);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 s = *reinterpret_cast<const float4 *>(&scale[c + h + j]);
+            const float4 b = *reinterpret_cast<const float4 *>(&bias[c + h + j]);
+            v[j] = fmaf((float)__float_as_int(v[j]) * xs, s.x, b.x);
+            v[j + 1] = fmaf((float)__float_as_int(v[j + 1]) * xs, s.y, b.y);
+            v[j + 2] = fmaf((float)__float_as_int(v[j + 2]) * xs, s.z, b.z);
+            v[j + 3] = fmaf((float)__float_as_int(v[j + 3]) * xs, s.w, b.w);
+          }
+          if (!ok) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = NAN;
+          }
+          constexpr int kPer = 16 / (int)sizeof(T);  // values per 16-byte chunk
+#pragma unroll
+          for (int j = 0; j < 32; j += kPer) {
+            const uint32_t at = stage + lane * 128 + ((((h + j) / kPer) ^ (lane & 7)) << 4);
+            if constexpr (sizeof(T) == 2)
+              tc::st_shared_v4(at, tc::pack_bf16(v[j], v[j + 1]), tc::pack_bf16(v[j + 2], v[j + 3]),
+                               tc::pack_bf16(v[j + 4], v[j + 5]), tc::pack_bf16(v[j + 6], v[j + 7]));
+            else
+              tc::st_shared_f4(at, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
+          }
+        }
+        __syncwarp();
+        T *y = static_cast<T *>(a.y) + (long long)m0 * a.N + n0 + c;
+        if (a.vec_ok) {  // four rows of 128 bytes per store
+          const int chunk = lane & 7, col = chunk * (16 / (int)sizeof(T));
+          if (n0 + c + col < a.N) {
+#pragma unroll
+            for (int r = lane >> 3; r < 32; r += 4) {
+              const float4 w = tc::ld_shared_f4(stage + r * 128 + ((chunk ^ (r & 7)) << 4));
+              if (r < rows) *reinterpret_cast<float4 *>(y + (long long)r * a.N + col) = w;
+            }
+          }
+        } else {
+          for (int r = 0; r < rows; ++r)
+#pragma unroll
+            for (int col = lane; col < kCols; col += 32) {
+              const uint32_t byte = col * (int)sizeof(T);
+              const uint32_t at = stage + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15);
+              if constexpr (sizeof(T) == 2) {
+                uint16_t w;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(at));
+                if (n0 + c + col < a.N) reinterpret_cast<uint16_t *>(y)[(long long)r * a.N + col] = w;
+              } else {
+                uint32_t w;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
+                if (n0 + c + col < a.N) reinterpret_cast<uint32_t *>(y)[(long long)r * a.N + col] = w;
+              }
+            }
+        }
+        __syncwarp();
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        arrive_cluster(map_rank(tc::smem_u32(&acc_empty[buf]), 0));
+        if (!ok) atomicExch(&g_timeout, 1);
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync();  // the pair's products and copies are done on both sides
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tmem_dealloc_pair(tmem, 2 * kPairN);
+  }
+}
+
+// ------------------------------------------------------------------ host side
 // Raises a kernel's dynamic shared-memory limit on the current device, once.
 template <typename F>
 cudaError_t allow_smem(F *kernel, int bytes, std::atomic<bool> (&set)[kMaxDevices]) {
@@ -163,14 +521,70 @@ cudaError_t allow_smem(F *kernel, int bytes, std::atomic<bool> (&set)[kMaxDevice
   return e;
 }
 
-template <typename T>
-int launch(const CUtensorMap &mx, const CUtensorMap &mw, const Args &a, cudaStream_t s) {
+int sm_count() {
+  static std::atomic<int> cached[kMaxDevices];
+  int dev = 0, v = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+  v = cached[dev].load();
+  if (!v) {
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) v = 148;
+    cached[dev].store(v);
+  }
+  return v;
+}
+
+template <typename T, int BT>
+int launch_split(const CUtensorMap &mx, const CUtensorMap &mw, const Args &a, cudaStream_t s) {
   static std::atomic<bool> set[kMaxDevices];
-  cudaError_t e = allow_smem(int8_tile_kernel<T>, kSmem, set);
+  cudaError_t e = allow_smem(split_kernel<T, BT>, Split<BT>::kBytes, set);
   if (e != cudaSuccess) return cuda_err("int8_linear", e);
-  const dim3 grid((unsigned)((a.N + kBN - 1) / kBN), (unsigned)((a.M + kBM - 1) / kBM));
-  int8_tile_kernel<T><<<grid, kThreads, kSmem, s>>>(mx, mw, a);
+  const int n_tiles = (a.N + kTileRows - 1) / kTileRows, m_tiles = (a.M + BT - 1) / BT;
+  // split K while every SM still gets at most one CTA and each CTA keeps two K steps
+  int S = 1;
+  while (S < kMaxSplit && 2LL * S * n_tiles * m_tiles <= sm_count() && a.k_steps >= 4 * S) S *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(n_tiles * S), (unsigned)m_tiles);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Split<BT>::kBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)S;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, split_kernel<T, BT>, mx, mw, a, S);
+  if (e != cudaSuccess) return cuda_err("int8_linear", e);
   return race::launched("int8_linear");
+}
+
+template <typename T>
+int launch_pair(const CUtensorMap &mx, const CUtensorMap &mw, const Args &a, cudaStream_t s) {
+  static std::atomic<bool> set[kMaxDevices];
+  const cudaError_t e = allow_smem(pair_kernel<T>, kPairSmem, set);
+  if (e != cudaSuccess) return cuda_err("int8_linear", e);
+  const long long tiles = (long long)a.m_tiles * a.n_tiles, pairs = sm_count() / 2;
+  pair_kernel<T><<<(unsigned)(2 * (tiles < pairs ? tiles : pairs)), kThreads, kPairSmem, s>>>(mx, mw, a);
+  return race::launched("int8_linear");
+}
+
+template <typename T>
+int launch(const int8_t *xq, int64_t x_stride, const int8_t *wq, int64_t w_stride, int64_t K, Args a, cudaStream_t s) {
+  a.m_tiles = (a.M + 255) / 256;
+  a.n_tiles = (a.N + kPairN - 1) / kPairN;
+  // The pair kernel once its tiles occupy half of the pairs
+  const bool pairs = a.M > 128 && (long long)a.m_tiles * a.n_tiles >= sm_count() / 4;
+  const int BT = pairs ? 128 : a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+  CUtensorMap mx, mw;
+  if (!race::make_byte_rows_map(&mx, xq, a.M, K, x_stride, BT) || !race::make_byte_rows_map(&mw, wq, a.N, K, w_stride, kTileRows))
+    return err(RACE_ERR_CUDA, "race_int8_linear: no tensor map for M=%lld, N=%lld", a.M, a.N);
+  if (pairs) return launch_pair<T>(mx, mw, a, s);
+  switch (BT) {
+    case 16: return launch_split<T, 16>(mx, mw, a, s);
+    case 32: return launch_split<T, 32>(mx, mw, a, s);
+    case 64: return launch_split<T, 64>(mx, mw, a, s);
+    default: return launch_split<T, 128>(mx, mw, a, s);
+  }
 }
 
 // race_set_status_check(1): wait for the stream and report a wait that gave up.
@@ -196,21 +610,22 @@ int race_int8_linear(const int8_t *xq, int64_t x_stride, const float *x_scale, c
                      void *stream) {
   if (!xq || !x_scale || !wq || !w_scale || !y) return err(RACE_ERR_ARG, "race_int8_linear: null pointer");
   if (dtype != RACE_F32 && dtype != RACE_BF16) return err(RACE_ERR_DTYPE, "race_int8_linear: dtype %lld", dtype);
-  // the grid's second dimension holds M / 128
-  if (M < 1 || N < 1 || M > 65535LL * kBM || N > 0x7fffff00LL)
+  // tile coordinates and the number of 128 x 128 tiles (times a split of 8) are 32-bit; a
+  // grid's second dimension holds the token tiles
+  if (M < 1 || N < 1 || M > (1 << 23) - 128 || N > (1 << 27) || ((M + 127) / 128) * ((N + 127) / 128) > (1 << 27))
     return err(RACE_ERR_SHAPE, "race_int8_linear: M=%lld or N=%lld out of range", M, N);
   if (K < 1 || K > kMaxK) return err(RACE_ERR_SHAPE, "race_int8_linear: K=%lld not in 1..%lld", K, kMaxK);
   if (x_stride < K || w_stride < K) return err(RACE_ERR_SHAPE, "race_int8_linear: row stride below K=%lld", K);
   if (((reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(wq) | (uintptr_t)x_stride | (uintptr_t)w_stride) & 15) ||
       ((reinterpret_cast<uintptr_t>(x_scale) | reinterpret_cast<uintptr_t>(w_scale) | reinterpret_cast<uintptr_t>(bias)) & 3))
     return err(RACE_ERR_ALIGN, "race_int8_linear: 8-bit rows must start at multiples of 16 bytes");
-  CUtensorMap mx, mw;
-  if (!race::make_byte_rows_map(&mx, xq, M, K, x_stride, kBM) || !race::make_byte_rows_map(&mw, wq, N, K, w_stride, kBN))
-    return err(RACE_ERR_CUDA, "race_int8_linear: no tensor map for M=%lld, N=%lld", M, N);
-  Args a{x_scale, w_scale, bias, y, M, N, (int)((K + kBK - 1) / kBK), 0, race::withhold_first_load() ? 1 : 0,
+  const int size = dtype == RACE_BF16 ? 2 : 4;
+  Args a{x_scale, w_scale, bias, y, (int)M, (int)N, (int)((K + kBK - 1) / kBK), 0, 0,
+         (N * size) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0, race::withhold_first_load() ? 1 : 0,
          race::current_wait_limit()};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int rc = dtype == RACE_BF16 ? launch<__nv_bfloat16>(mx, mw, a, s) : launch<float>(mx, mw, a, s);
+  const int rc = dtype == RACE_BF16 ? launch<__nv_bfloat16>(xq, x_stride, wq, w_stride, K, a, s)
+                                    : launch<float>(xq, x_stride, wq, w_stride, K, a, s);
   return rc == RACE_OK ? check_status(s) : rc;
 }
 
