@@ -80,12 +80,13 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a, uint64_t b, 
         : "memory");
 }
 
-// One stage's products: 128 bytes of K in steps of 32.
+// One stage's products: 128 bytes of K in steps of 32 (2 in a descriptor's address field,
+// which holds 16-byte units and does not carry: stages start at multiples of 1024).
 template <int CG>
 __device__ __forceinline__ void mma_stage(uint32_t d_tmem, uint32_t sa, uint32_t sb, uint32_t idesc, bool first) {
+  const uint64_t da = tc::sdesc(sa, 16, 1024), db = tc::sdesc(sb, 16, 1024);
 #pragma unroll
-  for (int j = 0; j < kBK / 32; ++j)
-    mma_i8<CG>(d_tmem, tc::sdesc(sa + 32 * j, 16, 1024), tc::sdesc(sb + 32 * j, 16, 1024), idesc, !(first && j == 0));
+  for (int j = 0; j < kBK / 32; ++j) mma_i8<CG>(d_tmem, da + 2 * j, db + 2 * j, idesc, !(first && j == 0));
 }
 
 // ---- cluster helpers
@@ -100,19 +101,14 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t smem_addr, uint32_t rank) 
   return r;
 }
 // every thread of every CTA of the cluster
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
-__device__ __forceinline__ int4 ld_cluster_i4(uint32_t addr) {
-  int4 v;
-  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ int ld_cluster_i(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster_i(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -149,15 +145,16 @@ __device__ __forceinline__ unsigned char *align_1k(unsigned char *p) {
 template <int BT>
 struct Split {
   static constexpr int kStageBytes = kTileBytes + BT * kBK;
-  // about 96 KB in flight per CTA, two CTAs per SM
-  static constexpr int kStages = BT <= 16 ? 5 : BT <= 32 ? 5 : BT <= 64 ? 4 : 3;
-  static constexpr int kSum = BT * kTileRows * 4;  // one CTA's integer sums, over the ring's stages
-  static constexpr int kBytes = (kStages * kStageBytes > kSum ? kStages * kStageBytes : kSum) + 1024;
+  // 72 to 128 KB on the way into a CTA; two CTAs per SM up to 64 tokens
+  static constexpr int kStages = BT <= 16 ? 5 : BT <= 32 ? 4 : BT <= 64 ? 3 : 4;
+  static constexpr int kRing = kStages * kStageBytes;
+  static constexpr int kBytes = kRing + BT * kTileRows * 4 + 1024;
   static constexpr int kCols = BT < 32 ? 32 : BT;  // TMEM columns (a power of two of at least 32)
 };
 
 // Grid (S * channel tiles, token tiles), clusters of S along x: rank r of a cluster takes the
-// r-th S-th of the K steps, then sums and stores channels [r, r + 1) * 128 / S of the tile.
+// r-th S-th of the K steps, and stores channels [r, r + 1) * 128 / S of the tile, to whose sums
+// every rank sends its part.
 template <typename T, int BT>
 __global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__ CUtensorMap mx,
                                                          const __grid_constant__ CUtensorMap mw, const Args a, const int S) {
@@ -166,128 +163,164 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__
   __shared__ uint64_t full[C::kStages], empty[C::kStages], done;
   __shared__ uint32_t tmem_slot;
   __shared__ int ctl[2];  // {abort flag, poll limit}
+  __shared__ int bad;     // some rank's sums are missing
+  __shared__ float xs[BT];
   unsigned char *ring = align_1k(smem_raw);
+  // [rank][token][channel of this CTA] integer sums
+  int *sums = reinterpret_cast<int *>(ring + C::kRing);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x % S, n0 = (int)(blockIdx.x / S) * kTileRows, m0 = blockIdx.y * BT;
+  const int width = kTileRows / S;  // channels this CTA stores: 16 to 128
+  const int tokens = min(BT, a.M - m0);
   const int k_begin = (int)((long long)a.k_steps * rank / S), k_end = (int)((long long)a.k_steps * (rank + 1) / S);
   const int steps = k_end - k_begin;
   volatile int *abort = ctl;
 
-  if (threadIdx.x == 0) {
+  // The producer lane sets the barriers up and has the first copies on their way before the
+  // rest of the block is ready.
+  int st = 0, issued = 0;
+  uint32_t parity = 1;  // a fresh barrier's last phase counts as done
+  auto load_next = [&]() {
+    unsigned char *sw = ring + st * C::kStageBytes;
+    tc::mbar_arrive_expect_tx(&full[st], C::kStageBytes);
+    tc::tma_load_2d(sw, &mw, &full[st], (k_begin + issued) * kBK, n0);
+    tc::tma_load_2d(sw + kTileBytes, &mx, &full[st], (k_begin + issued) * kBK, m0);
+    ++issued;
+    if (++st == C::kStages) st = 0, parity ^= 1;
+  };
+  const int wanted = a.withhold ? 0 : steps;
+  if (threadIdx.x == 64) {
     tc::prefetch_tmap(&mx);
     tc::prefetch_tmap(&mw);
-    ctl[0] = 0;
-    ctl[1] = (int)a.wait_limit;
+  }
+  if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
     }
     tc::mbar_init(&done, 1);
+    ctl[0] = 0;
+    ctl[1] = (int)a.wait_limit;
+    bad = 0;
     tc::fence_mbar_init();
+    while (issued < wanted && issued < C::kStages) load_next();
   }
   if (warp == 1) tc::tmem_alloc(&tmem_slot, C::kCols);
+  for (int t = (int)threadIdx.x - 64; t < tokens; t += kThreads - 64)
+    if (t >= 0) xs[t] = __ldg(a.xs + m0 + t);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  if (S > 1) cluster_arrive();  // this block runs, and its `bad` is clear
 
   if (warp == 0) {
     if (lane == 0) {
-      int issued = 0;
-      for (int k = 0; k < (a.withhold ? 0 : steps); ++k) {
-        const int st = k % C::kStages, use = k / C::kStages;
-        if (use && !tc::mbar_wait(&empty[st], (use - 1) & 1, abort)) break;
-        unsigned char *sw = ring + st * C::kStageBytes;
-        tc::mbar_arrive_expect_tx(&full[st], C::kStageBytes);
-        tc::tma_load_2d(sw, &mw, &full[st], (k_begin + k) * kBK, n0);
-        tc::tma_load_2d(sw + kTileBytes, &mx, &full[st], (k_begin + k) * kBK, m0);
-        issued = k + 1;
+      while (issued < wanted) {
+        if (!tc::mbar_wait(&empty[st], parity, abort)) break;
+        load_next();
       }
       if (*abort)  // no copy may land after the block has gone
         for (int k = issued > C::kStages ? issued - C::kStages : 0; k < issued; ++k)
           tc::mbar_wait_drain(&full[k % C::kStages], (k / C::kStages) & 1);
     }
     __syncwarp();
+    if (S > 1) cluster_wait();
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t id = idesc_i8(kTileRows, BT);
+      int at = 0;
+      uint32_t phase = 0;
+      bool ready = false;  // as in pair_kernel: the next stage's wait runs behind this one's issue
       for (int k = 0; k < steps; ++k) {
-        const int st = k % C::kStages;
-        if (!tc::mbar_wait(&full[st], (k / C::kStages) & 1, abort)) break;
+        if (!ready && !tc::mbar_wait(&full[at], phase, abort)) break;
         tc::tc_fence_after();
-        const uint32_t sw = tc::smem_u32(ring + st * C::kStageBytes);
+        const int now = at;
+        if (++at == C::kStages) at = 0, phase ^= 1;
+        ready = tc::mbar_try_wait(&full[at], phase);
+        const uint32_t sw = tc::smem_u32(ring) + now * C::kStageBytes;
         mma_stage<1>(tmem, sw, sw + kTileBytes, id, k == 0);
-        tc::mma_commit(&empty[st]);
+        tc::mma_commit(&empty[now]);
       }
       tc::mma_commit(&done);
       if (*abort) tc::mbar_wait_drain(&done, 0);
     }
     __syncwarp();
+    if (S > 1) cluster_wait();
   } else {
-    // this CTA's sums as [token][channel] integers, over the ring (all its copies are consumed)
+    // send this rank's sums to the blocks that store them: a thread has one channel
     const int quarter = warp & 3;  // the TMEM lanes a warp may read
+    const int c = quarter * 32 + lane, owner = c / width;
+    if (S > 1) cluster_wait();
     const bool ok = tc::warp_all(tc::mbar_wait(&done, 0, abort) && !*abort);
     tc::tc_fence_after();
-    int *sum = reinterpret_cast<int *>(ring) + quarter * 32 + lane;
-    const bool live = ok && steps > 0;
+    const uint32_t to = map_rank(tc::smem_u32(sums + (rank * BT) * width + c - owner * width), owner);
+    const uint32_t row = 4 * width;
 #pragma unroll
-    for (int c = 0; c < BT; c += 16) {
-      float v[16];
-      tc::tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
-      tc::tmem_wait_ld();
-      if (ok) {
+    for (int t0 = 0; t0 < BT; t0 += 16) {
+      if (t0 < tokens) {
+        float v[16];
+        tc::tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + t0, v);
+        tc::tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sum[(c + j) * kTileRows] = live ? __float_as_int(v[j]) : 0;
+        for (int t = 0; t < 16; ++t)
+          if (t0 + t < tokens) st_cluster_i(to + (t0 + t) * row, __float_as_int(v[t]));
       }
-      __syncwarp();
     }
+    if (!ok && lane < S) st_cluster_i(map_rank(tc::smem_u32(&bad), lane), 1);
     tc::tc_fence_before();
+    __syncwarp();
   }
-  cluster_sync();
+  if (S > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
 
-  // add the cluster's sums for this CTA's channels, scale and store
-  bool ok = true;
-  for (int r = 0; r < S; ++r) ok = ok && ld_cluster_i(map_rank(tc::smem_u32(&ctl[0]), r)) == 0;
-  const int width = kTileRows / S, c0 = rank * width;  // channels of this CTA: 16 to 128
-  const int quads = width / 4;
-  const uint32_t base = tc::smem_u32(ring) + 4 * c0;
-  for (int e = threadIdx.x; e < BT * quads; e += kThreads) {
-    const int t = e / quads, c = 4 * (e % quads);
-    const int m = m0 + t, n = n0 + c0 + c;
-    if (m >= a.M || n >= a.N) continue;
-    int4 acc = make_int4(0, 0, 0, 0);
-    const uint32_t at = base + 4 * (t * kTileRows + c);
-#pragma unroll
-    for (int r = 0; r < kMaxSplit; ++r)
-      if (r < S) {
-        const int4 v = ld_cluster_i4(map_rank(at, r));
-        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-      }
-    const float xs = __ldg(a.xs + m);
-    const int q[4] = {acc.x, acc.y, acc.z, acc.w};
-    float f[4];
+  // add the ranks' sums, scale and store: a thread has four channels and every `step`-th token
+  const bool ok = *(volatile int *)&bad == 0;
+  const int quads = width / 4, q = threadIdx.x % quads, step = kThreads / quads;
+  const int n = n0 + rank * width + 4 * q;
+  if (n < a.N) {
+    float ws[4], bias[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int nn = min(n + j, a.N - 1);
-      f[j] = (float)q[j] * xs * __ldg(a.ws + nn);
-      if (a.bias) f[j] += __ldg(a.bias + nn);
-      if (!ok) f[j] = NAN;
+      ws[j] = __ldg(a.ws + nn);
+      bias[j] = a.bias ? __ldg(a.bias + nn) : 0.f;
     }
-    T *y = static_cast<T *>(a.y) + (long long)m * a.N + n;
-    if (a.vec_ok) {  // N is a multiple of 16 bytes' worth of values: n + 3 < N too
-      if constexpr (sizeof(T) == 2)
-        *reinterpret_cast<uint2 *>(y) = make_uint2(tc::pack_bf16(f[0], f[1]), tc::pack_bf16(f[2], f[3]));
-      else
-        *reinterpret_cast<float4 *>(y) = make_float4(f[0], f[1], f[2], f[3]);
-    } else {
+    T *y = static_cast<T *>(a.y) + (long long)m0 * a.N + n;
+#pragma unroll 4
+    for (int t = threadIdx.x / quads; t < tokens; t += step) {
+      const int4 *from = reinterpret_cast<const int4 *>(sums + t * width + 4 * q);
+      int4 acc = from[0];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < a.N) y[j] = race::from_f<T>(f[j]);
+      for (int r = 1; r < kMaxSplit; ++r)
+        if (r < S) {
+          const int4 v = from[r * (BT * width / 4)];
+          acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+        }
+      const float s = xs[t];
+      float f[4] = {fmaf((float)acc.x * s, ws[0], bias[0]), fmaf((float)acc.y * s, ws[1], bias[1]),
+                    fmaf((float)acc.z * s, ws[2], bias[2]), fmaf((float)acc.w * s, ws[3], bias[3])};
+      if (!ok) f[0] = f[1] = f[2] = f[3] = NAN;
+      T *o = y + (long long)t * a.N;
+      if (a.vec_ok) {  // N is a multiple of 16 bytes' worth of values: n + 3 < N too
+        if constexpr (sizeof(T) == 2)
+          *reinterpret_cast<uint2 *>(o) = make_uint2(tc::pack_bf16(f[0], f[1]), tc::pack_bf16(f[2], f[3]));
+        else
+          *reinterpret_cast<float4 *>(o) = make_float4(f[0], f[1], f[2], f[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < a.N) o[j] = race::from_f<T>(f[j]);
+      }
     }
   }
   if (!ok && threadIdx.x == 0) atomicExch(&g_timeout, 1);
-  cluster_sync();  // nobody leaves while its sums are read
   if (warp == 1) {
+    __syncwarp();
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, C::kCols);
   }
@@ -297,8 +330,17 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__
 constexpr int kPairStages = 6;
 constexpr int kPairStageBytes = 2 * kTileBytes;
 constexpr int kPairN = 256;               // channels per tile and accumulator columns
-constexpr int kStageOut = 4 * 32 * 128;   // per epilogue warp: 32 rows x 128 bytes on their way out
-constexpr int kPairSmem = kPairStages * kPairStageBytes + kStageOut + 1024;
+constexpr int kOutWarps = 8;              // epilogue warps: two per TMEM lane quarter, half of the columns each
+constexpr int kPairThreads = 64 + 32 * kOutWarps;
+// everything the pair kernel keeps in shared memory (227 KB per CTA allow one more kilobyte)
+struct PairSmem {
+  unsigned char ring[kPairStages][kPairStageBytes];
+  unsigned char out[kOutWarps][32 * 128];  // 32 rows x 128 bytes on their way out
+  float scale[kPairN], bias[kPairN];       // of the tile's channels
+  uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2], drained;
+  uint32_t tmem_slot;
+  int ctl[2];  // {abort flag, poll limit}
+};
 constexpr int kGroupM = 8;                // token tiles that share their weight tiles in L2
 
 // The t-th tile: groups of kGroupM token tiles, inside a group the token tile varies fastest.
@@ -311,15 +353,14 @@ __device__ __forceinline__ void tile_at(const Args &a, int t, int &mt, int &nt) 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) __cluster_dims__(2, 1, 1)
+__global__ void __launch_bounds__(kPairThreads) __cluster_dims__(2, 1, 1)
 pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const Args a) {
-  extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2], drained;
-  __shared__ uint32_t tmem_slot;
-  __shared__ int ctl[2];  // {abort flag, poll limit}
-  __shared__ __align__(16) float scale[kPairN], bias[kPairN];
-  unsigned char *ring = align_1k(smem_raw);
-  unsigned char *out_stage = ring + kPairStages * kPairStageBytes;
+  extern __shared__ __align__(1024) unsigned char pair_smem[];
+  PairSmem &sm = *reinterpret_cast<PairSmem *>(pair_smem);
+  uint64_t *full = sm.full, *empty = sm.empty, *acc_full = sm.acc_full, *acc_empty = sm.acc_empty;
+  unsigned char *ring = sm.ring[0];
+  float *scale = sm.scale, *bias = sm.bias;
+  int *ctl = sm.ctl;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int tiles = a.m_tiles * a.n_tiles;
@@ -328,7 +369,7 @@ pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUte
   if (threadIdx.x == 0) {
     tc::prefetch_tmap(&mx);
     tc::prefetch_tmap(&mw);
-    ctl[0] = 0;
+    ctl[0] = (tc::smem_u32(ring) & 1023) != 0;  // the swizzled tiles start at multiples of 1024
     ctl[1] = (int)a.wait_limit;
     for (int i = 0; i < kPairStages; ++i) {
       tc::mbar_init(&full[i], 1);
@@ -336,80 +377,89 @@ pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUte
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&acc_full[i], 1);
-      tc::mbar_init(&acc_empty[i], 8);  // the pair's epilogue warps
+      tc::mbar_init(&acc_empty[i], 2 * kOutWarps);  // the pair's epilogue warps
     }
-    tc::mbar_init(&drained, 1);
+    tc::mbar_init(&sm.drained, 1);
     tc::fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc_pair(&tmem_slot, 2 * kPairN);
+  if (warp == 1) tmem_alloc_pair(&sm.tmem_slot, 2 * kPairN);
   tc::tc_fence_before();
   cluster_sync();  // both CTAs' barriers exist
   tc::tc_fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = sm.tmem_slot;
 
   if (warp == 0) {
     if (lane == 0 && !a.withhold) {
-      long long step = 0;  // stages filled so far, over all tiles
-      bool go = true;
+      int st = 0, filled = 0;     // the next stage, and how many are filled or were
+      uint32_t parity = 1;        // of the wait for a free stage: a fresh barrier's last phase counts as done
+      bool go = true, ready = true;
+      const uint32_t leader_full = map_rank(tc::smem_u32(&full[0]), 0);
       for (int t = pair; go && t < tiles; t += pairs) {
         int mt, nt;
         tile_at(a, t, mt, nt);
         const int m = mt * 256 + rank * kTileRows, n = nt * kPairN + rank * kTileRows;
-        for (int k = 0; k < a.k_steps; ++k, ++step) {
-          const int st = (int)(step % kPairStages);
-          const long long use = step / kPairStages;
-          if (use && !tc::mbar_wait(&empty[st], (uint32_t)(use - 1) & 1, abort)) {
+        for (int k = 0; k < a.k_steps; ++k) {
+          if (!ready && !tc::mbar_wait(&empty[st], parity, abort)) {
             go = false;
             break;
           }
-          const uint32_t sa = tc::smem_u32(ring + st * kPairStageBytes);
-          const uint32_t bar = map_rank(tc::smem_u32(&full[st]), 0);
+          const int now = st;
+          if (++st == kPairStages) st = 0, parity ^= 1;
+          ready = tc::mbar_try_wait(&empty[st], parity);  // answers while this stage's copies are issued
+          const uint32_t sa = tc::smem_u32(ring) + now * kPairStageBytes;
+          const uint32_t bar = leader_full + now * 8;
           // the leader's barrier counts both CTAs' bytes; the peer's may land first
-          if (rank == 0) tc::mbar_arrive_expect_tx(&full[st], 2 * kPairStageBytes);
+          if (rank == 0) tc::mbar_arrive_expect_tx(&full[now], 2 * kPairStageBytes);
           tma_load_pair(sa, &mx, bar, k * kBK, m);
           tma_load_pair(sa + kTileBytes, &mw, bar, k * kBK, n);
+          filled = min(filled + 1, kPairStages);
         }
       }
-      if (*abort && rank == 0) {  // both CTAs' copies must have landed before either leaves
-        const long long first = step > kPairStages ? step - kPairStages : 0;
-        for (long long s = first; s < step; ++s)
-          tc::mbar_wait_drain(&full[s % kPairStages], (uint32_t)(s / kPairStages) & 1);
-      }
+      if (*abort && rank == 0)  // both CTAs' copies must have landed before either leaves
+        for (; filled > 0; --filled) {  // newest first
+          if (st-- == 0) st = kPairStages - 1, parity ^= 1;
+          tc::mbar_wait_drain(&full[st], parity ^ 1);
+        }
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       constexpr uint32_t id = idesc_i8(256, kPairN);
-      long long step = 0;
-      int i = 0;
-      bool go = true;
-      for (int t = pair; go && t < tiles; t += pairs, ++i) {
-        const int buf = i & 1, use = i >> 1;
-        if (use && !tc::mbar_wait(&acc_empty[buf], (use - 1) & 1, abort)) break;
+      int st = 0, buf = 0;
+      uint32_t parity = 0, acc_parity = 1;
+      // Even on a completed barrier a wait answers only after some 300 cycles, so each asks for
+      // the next stage before it issues this one's work: 410 -> 355 us at 8192^3 (827 -> 650
+      // cycles per stage on this thread, of which the products take 512).
+      bool go = true, ready = false;
+      for (int t = pair; go && t < tiles; t += pairs) {
+        if (!tc::mbar_wait(&acc_empty[buf], acc_parity, abort)) break;
         tc::tc_fence_after();
-        for (int k = 0; k < a.k_steps; ++k, ++step) {
-          const int st = (int)(step % kPairStages);
-          if (!tc::mbar_wait(&full[st], (uint32_t)(step / kPairStages) & 1, abort)) {
+        for (int k = 0; k < a.k_steps; ++k) {
+          if (!ready && !tc::mbar_wait(&full[st], parity, abort)) {
             go = false;
             break;
           }
           tc::tc_fence_after();
-          const uint32_t sa = tc::smem_u32(ring + st * kPairStageBytes);
+          const int now = st;
+          if (++st == kPairStages) st = 0, parity ^= 1;
+          ready = tc::mbar_try_wait(&full[st], parity);
+          const uint32_t sa = tc::smem_u32(ring) + now * kPairStageBytes;
           mma_stage<2>(tmem + buf * kPairN, sa, sa + kTileBytes, id, k == 0);
-          commit_pair(&empty[st]);
+          commit_pair(&empty[now]);
         }
         if (go) commit_pair(&acc_full[buf]);
+        if (++buf == 2) buf = 0, acc_parity ^= 1;
       }
       if (*abort) {
-        commit_pair(&drained);
-        tc::mbar_wait_drain(&drained, 0);
+        commit_pair(&sm.drained);
+        tc::mbar_wait_drain(&sm.drained, 0);
       }
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3;
-    const int et = threadIdx.x - 64;  // 0..127 over the epilogue warps
-    const uint32_t stage = tc::smem_u32(out_stage) + quarter * (32 * 128);
+    const int quarter = warp & 3, half = (warp - 2) >> 2;  // the TMEM lanes a warp may read; its columns
+    const int et = threadIdx.x - 64;                       // over the epilogue warps
+    const uint32_t stage = tc::smem_u32(sm.out[warp - 2]);
     constexpr int kCols = 128 / (int)sizeof(T);  // columns per 128-byte output row
     int i = 0;
     for (int t = pair; t < tiles; t += pairs, ++i) {
@@ -417,49 +467,49 @@ pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUte
       tile_at(a, t, mt, nt);
       const int buf = i & 1, use = i >> 1;
       const int m0 = mt * 256 + rank * kTileRows + quarter * 32, n0 = nt * kPairN;
-      tc::named_bar_sync(1, 128);  // the last tile's scales are read
-      for (int c = et; c < kPairN; c += 128) {
-        const int n = min(n0 + c, a.N - 1);
-        scale[c] = __ldg(a.ws + n);
-        bias[c] = a.bias ? __ldg(a.bias + n) : 0.f;
+      tc::named_bar_sync(1, 32 * kOutWarps);  // the last tile's scales are read
+      {
+        static_assert(kPairN == 32 * kOutWarps, "one channel per epilogue thread");
+        const int n = min(n0 + et, a.N - 1);
+        scale[et] = __ldg(a.ws + n);
+        bias[et] = a.bias ? __ldg(a.bias + n) : 0.f;
       }
       const int m = m0 + lane;
       const float xs = m < a.M ? __ldg(a.xs + m) : 0.f;
-      tc::named_bar_sync(1, 128);
+      tc::named_bar_sync(1, 32 * kOutWarps);
       const bool ok = tc::warp_all(!*abort && tc::mbar_wait(&acc_full[buf], use & 1, abort));
       tc::tc_fence_after();
       const int rows = min(32, a.M - m0);
 #pragma unroll 1
-      for (int c = 0; c < kPairN; c += kCols) {
+      for (int c = half * (kPairN / 2); c < (half + 1) * (kPairN / 2); c += kCols) {
+        float v[kCols];
+#pragma unroll
+        for (int h = 0; h < kCols; h += 32)
+          tc::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + buf * kPairN + c + h, *reinterpret_cast<float(*)[32]>(&v[h]));
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < kCols; j += 4) {
+          const float4 s = *reinterpret_cast<const float4 *>(&scale[c + j]);
+          const float4 b = *reinterpret_cast<const float4 *>(&bias[c + j]);
+          v[j] = fmaf((float)__float_as_int(v[j]) * xs, s.x, b.x);
+          v[j + 1] = fmaf((float)__float_as_int(v[j + 1]) * xs, s.y, b.y);
+          v[j + 2] = fmaf((float)__float_as_int(v[j + 2]) * xs, s.z, b.z);
+          v[j + 3] = fmaf((float)__float_as_int(v[j + 3]) * xs, s.w, b.w);
+        }
+        if (!ok) {
+#pragma unroll
+          for (int j = 0; j < kCols; ++j) v[j] = NAN;
+        }
         // a row of 128 output bytes per lane, its 16-byte chunks swizzled by the row
+        constexpr int kPer = 16 / (int)sizeof(T);  // values per 16-byte chunk
 #pragma unroll
-        for (int h = 0; h < kCols; h += 32) {
-          float v[32];
-          tc::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + buf * kPairN + c + h, v);
-          tc::tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 s = *reinterpret_cast<const float4 *>(&scale[c + h + j]);
-            const float4 b = *reinterpret_cast<const float4 *>(&bias[c + h + j]);
-            v[j] = fmaf((float)__float_as_int(v[j]) * xs, s.x, b.x);
-            v[j + 1] = fmaf((float)__float_as_int(v[j + 1]) * xs, s.y, b.y);
-            v[j + 2] = fmaf((float)__float_as_int(v[j + 2]) * xs, s.z, b.z);
-            v[j + 3] = fmaf((float)__float_as_int(v[j + 3]) * xs, s.w, b.w);
-          }
-          if (!ok) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = NAN;
-          }
-          constexpr int kPer = 16 / (int)sizeof(T);  // values per 16-byte chunk
-#pragma unroll
-          for (int j = 0; j < 32; j += kPer) {
-            const uint32_t at = stage + lane * 128 + ((((h + j) / kPer) ^ (lane & 7)) << 4);
-            if constexpr (sizeof(T) == 2)
-              tc::st_shared_v4(at, tc::pack_bf16(v[j], v[j + 1]), tc::pack_bf16(v[j + 2], v[j + 3]),
-                               tc::pack_bf16(v[j + 4], v[j + 5]), tc::pack_bf16(v[j + 6], v[j + 7]));
-            else
-              tc::st_shared_f4(at, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
-          }
+        for (int j = 0; j < kCols; j += kPer) {
+          const uint32_t at = stage + lane * 128 + (((j / kPer) ^ (lane & 7)) << 4);
+          if constexpr (sizeof(T) == 2)
+            tc::st_shared_v4(at, tc::pack_bf16(v[j], v[j + 1]), tc::pack_bf16(v[j + 2], v[j + 3]),
+                             tc::pack_bf16(v[j + 4], v[j + 5]), tc::pack_bf16(v[j + 6], v[j + 7]));
+          else
+            tc::st_shared_f4(at, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
         }
         __syncwarp();
         T *y = static_cast<T *>(a.y) + (long long)m0 * a.N + n0 + c;
@@ -539,9 +589,13 @@ int launch_split(const CUtensorMap &mx, const CUtensorMap &mw, const Args &a, cu
   cudaError_t e = allow_smem(split_kernel<T, BT>, Split<BT>::kBytes, set);
   if (e != cudaSuccess) return cuda_err("int8_linear", e);
   const int n_tiles = (a.N + kTileRows - 1) / kTileRows, m_tiles = (a.M + BT - 1) / BT;
-  // split K while every SM still gets at most one CTA and each CTA keeps two K steps
+  // Split K while each CTA keeps two K steps and the CTAs fit on the SMs at once: two per SM up
+  // to 64 tokens (64 x 16384 x 2048: 12.6 us with 256 CTAs, 13.8 with 128), one with 128, whose
+  // sums to exchange cost more than the second CTA gains (256 x 2048 x 2048: 8.3 us with one,
+  // 18.7 with two).
+  const int room = sm_count() * (BT <= 64 ? 2 : 1);
   int S = 1;
-  while (S < kMaxSplit && 2LL * S * n_tiles * m_tiles <= sm_count() && a.k_steps >= 4 * S) S *= 2;
+  while (S < kMaxSplit && 2LL * S * n_tiles * m_tiles <= room && a.k_steps >= 4 * S) S *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(n_tiles * S), (unsigned)m_tiles);
   cfg.blockDim = dim3(kThreads);
@@ -552,7 +606,7 @@ int launch_split(const CUtensorMap &mx, const CUtensorMap &mw, const Args &a, cu
   attr.val.clusterDim.x = (unsigned)S;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = S > 1;
   e = cudaLaunchKernelEx(&cfg, split_kernel<T, BT>, mx, mw, a, S);
   if (e != cudaSuccess) return cuda_err("int8_linear", e);
   return race::launched("int8_linear");
@@ -561,10 +615,10 @@ int launch_split(const CUtensorMap &mx, const CUtensorMap &mw, const Args &a, cu
 template <typename T>
 int launch_pair(const CUtensorMap &mx, const CUtensorMap &mw, const Args &a, cudaStream_t s) {
   static std::atomic<bool> set[kMaxDevices];
-  const cudaError_t e = allow_smem(pair_kernel<T>, kPairSmem, set);
+  const cudaError_t e = allow_smem(pair_kernel<T>, sizeof(PairSmem), set);
   if (e != cudaSuccess) return cuda_err("int8_linear", e);
   const long long tiles = (long long)a.m_tiles * a.n_tiles, pairs = sm_count() / 2;
-  pair_kernel<T><<<(unsigned)(2 * (tiles < pairs ? tiles : pairs)), kThreads, kPairSmem, s>>>(mx, mw, a);
+  pair_kernel<T><<<(unsigned)(2 * (tiles < pairs ? tiles : pairs)), kPairThreads, sizeof(PairSmem), s>>>(mx, mw, a);
   return race::launched("int8_linear");
 }
 
