@@ -591,11 +591,12 @@ int launch_split(const CUtensorMap &mx, const CUtensorMap &mw, const Args &a, cu
   const int n_tiles = (a.N + kTileRows - 1) / kTileRows, m_tiles = (a.M + BT - 1) / BT;
   // Split K while each CTA keeps two K steps and the CTAs fit on the SMs at once: two per SM up
   // to 64 tokens (64 x 16384 x 2048: 12.6 us with 256 CTAs, 13.8 with 128), one with 128, whose
-  // sums to exchange cost more than the second CTA gains (256 x 2048 x 2048: 8.3 us with one,
-  // 18.7 with two).
+  // sums to exchange cost more than more CTAs gain (256 x 2048 x 2048: 8.3 us with one per SM,
+  // 18.7 with two; 128 x 2048 x 2048: 8.1 us split four ways, 13.0 eight).
   const int room = sm_count() * (BT <= 64 ? 2 : 1);
   int S = 1;
-  while (S < kMaxSplit && 2LL * S * n_tiles * m_tiles <= room && a.k_steps >= 4 * S) S *= 2;
+  constexpr int kMost = BT <= 64 ? kMaxSplit : kMaxSplit / 2;
+  while (S < kMost && 2LL * S * n_tiles * m_tiles <= room && a.k_steps >= 4 * S) S *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(n_tiles * S), (unsigned)m_tiles);
   cfg.blockDim = dim3(kThreads);

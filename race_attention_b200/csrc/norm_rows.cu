@@ -18,6 +18,8 @@
 #include <math.h>
 #include <stdio.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 #include "internal.h"
 
@@ -40,6 +42,7 @@ struct RowArgs {
   long long rows, x_stride, r_stride, q_stride;
   int K, w_bf16;
   float eps;
+  int q_vec = 0;  // 8-byte stores of 8-bit rows
 };
 
 __device__ __forceinline__ float weight_at(const void *w, int w_bf16, long long i) {
@@ -72,24 +75,381 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t v, float *red) {
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// q = round(y / scale).  The product with 127 / amax stands for the division except
-// where that factor would overflow (rows of magnitudes near the smallest floats).
+// q = round(127 y / amax).  Rows of magnitudes near the smallest floats are first scaled by
+// 2^100 (`lift`), so that 127 / amax does not overflow.  A row of zeros gives 0 * infinity, and
+// the conversion of a NaN to an integer 0.
 struct Quantiser {
-  float scale, inv;
-  bool tiny;
+  float scale, lift, inv;
   __device__ __forceinline__ explicit Quantiser(uint32_t amax_bits) {
     const float amax = __uint_as_float(amax_bits);
     scale = amax / 127.f;
-    tiny = amax < 1e-30f;
-    inv = tiny ? 0.f : 127.f / amax;
+    lift = amax < 1e-30f ? 0x1p100f : 1.f;
+    inv = 127.f / (amax * lift);
   }
-  __device__ __forceinline__ int operator()(float y) const {
-    if (tiny) return scale > 0.f ? __float2int_rn(y / scale) : 0;
-    return __float2int_rn(y * inv);
+  __device__ __forceinline__ int operator()(float lifted) const { return __float2int_rn(lifted * inv); }
+};
+
+// (the approximate quotient is 0 where the denominator passes 2^126: the product is then 0 too)
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+
+// ---------------------------------------------------------------- rows in registers
+// A group of G threads owns a row and holds it in registers, so the row is read once however
+// many passes its statistics take: thread tid's i-th vector is 8 values, from (i G + tid) 8 on.
+// Three layouts, told apart by where the rows lie in the 16-byte granules of memory:
+//   kAligned  every row of every tensor starts at a granule and K is a multiple of 8
+//   kSkewed   the tensors' rows start equally far into a granule (odd widths): vector j is
+//             values 8 j - off .. 8 j - off + 7, whole granules but at a row's ends.  A group
+//             only takes rows with one and the same off (their numbers differ by a multiple
+//             of 8), so its columns stay put and their weights are loaded once.
+//   kShifted  neither (the halves of SwiGLU rows of odd width): a vector is put together from
+//             the granules that hold it
+enum Layout { kAligned = 0, kSkewed = 1, kShifted = 2 };
+
+template <typename T>
+constexpr int kWords = 2 * (int)sizeof(T);  // 32-bit words of 8 values
+template <typename T>
+constexpr int kPerG = 16 / (int)sizeof(T);  // values per 16-byte granule
+
+__device__ __forceinline__ uint4 ldg16(const void *p) { return __ldg(static_cast<const uint4 *>(p)); }
+
+template <typename T>
+__device__ __forceinline__ int misalign(const T *p) {  // values past a granule's start
+  return (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+}
+
+// c[i] = the words that start `off` values further on
+template <typename T, int N>
+__device__ __forceinline__ void shift_down(uint32_t (&c)[N], int off) {
+  if constexpr (sizeof(T) == 2) {
+    if (off & 4) {
+#pragma unroll
+      for (int i = 0; i + 2 < N; ++i) c[i] = c[i + 2];
+    }
+    if (off & 2) {
+#pragma unroll
+      for (int i = 0; i + 1 < N; ++i) c[i] = c[i + 1];
+    }
+    if (off & 1) {
+#pragma unroll
+      for (int i = 0; i + 1 < N; ++i) c[i] = __funnelshift_r(c[i], c[i + 1], 16);
+    }
+  } else {
+    if (off & 2) {
+#pragma unroll
+      for (int i = 0; i + 2 < N; ++i) c[i] = c[i + 2];
+    }
+    if (off & 1) {
+#pragma unroll
+      for (int i = 0; i + 1 < N; ++i) c[i] = c[i + 1];
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void words_to_floats(const uint32_t *u, float *f) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(u[i] << 16);
+      f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(u[i]);
+  }
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <typename T>
+__device__ __forceinline__ void floats_to_words(const float *f, uint32_t *u) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = pack2(f[2 * i], f[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(f[i]);
+  }
+}
+
+// Eight values as they came from memory, unpacked where they are used so that many are in
+// flight at once.
+template <typename T, int LAYOUT>
+struct Vec8 {
+  static constexpr int N = kWords<T> + (LAYOUT == kShifted ? 4 : 0);
+  uint32_t c[N];
+  int off;
+
+  template <int M>
+  __device__ __forceinline__ void granules(const T *g) {
+#pragma unroll
+    for (int i = 0; i < M; i += 4) {
+      const uint4 v = ldg16(reinterpret_cast<const uint32_t *>(g) + i);
+      c[i] = v.x, c[i + 1] = v.y, c[i + 2] = v.z, c[i + 3] = v.w;
+    }
+  }
+  __device__ __forceinline__ void singles(const T *p, int e, int K) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (e + k >= 0 && e + k < K) {
+        if constexpr (sizeof(T) == 2)
+          c[k / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(p) + e + k) << (16 * (k & 1));
+        else
+          c[k] = __ldg(reinterpret_cast<const uint32_t *>(p) + e + k);
+      }
+  }
+  // Values e .. e + 7 of the row p of K values, of a tensor whose values lie in [begin, end).
+  // Granules that reach past the row's ends are read whole where they lie in the tensor (the
+  // other values are dropped by unpack), so that no single loads are waited for.
+  __device__ __forceinline__ void load(const T *p, int e, int K, const T *begin, const T *end) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[i] = 0;
+    if constexpr (LAYOUT == kAligned) {
+      if (e < K) granules<N>(p + e);
+    } else {
+      const int row_off = LAYOUT == kShifted ? misalign(p) : 0;
+      const T *g = p + e - row_off;
+      off = row_off;
+      if (e > -8 && e < K) {
+        if (g >= begin && g + N * 4 / (int)sizeof(T) <= end) {
+          granules<N>(g);
+        } else {
+          off = 0;
+          singles(p, e, K);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack(float *f, int e, int K) const {
+    if constexpr (LAYOUT == kShifted) {
+      uint32_t d[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) d[i] = c[i];
+      shift_down<T>(d, off);
+      words_to_floats<T>(d, f);
+    } else {
+      words_to_floats<T>(c, f);
+    }
+    if (LAYOUT != kAligned && (e < 0 || e + 8 > K)) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (e + k < 0 || e + k >= K) f[k] = 0.f;
+    }
   }
 };
 
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }
+// Stores values e .. e + 7 (those the row has).
+template <typename T, int LAYOUT>
+__device__ __forceinline__ void store8(T *p, int e, int K, const float *f) {
+  if (LAYOUT == kAligned ? e < K : e >= 0 && e + 8 <= K) {
+    uint32_t c[kWords<T>];
+    floats_to_words<T>(f, c);
+#pragma unroll
+    for (int i = 0; i < kWords<T>; i += 4)
+      reinterpret_cast<uint4 *>(p + e)[i / 4] = make_uint4(c[i], c[i + 1], c[i + 2], c[i + 3]);
+  } else if (LAYOUT != kAligned && e < K) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (e + k >= 0 && e + k < K) p[e + k] = from_f<T>(f[k]);
+  }
+}
+
+// weights e .. e + 7 (1 where there are none); `whole`: they are a vector from a granule on
+__device__ __forceinline__ void weights8(const void *w, int w_bf16, bool whole, int e, int K, float *f) {
+  if (w && whole) {
+    uint32_t u[8];
+    const uint32_t *g = w_bf16 ? reinterpret_cast<const uint32_t *>(static_cast<const __nv_bfloat16 *>(w) + e)
+                               : reinterpret_cast<const uint32_t *>(static_cast<const float *>(w) + e);
+    const uint4 v = ldg16(g);
+    u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
+    if (w_bf16) {
+      words_to_floats<__nv_bfloat16>(u, f);
+    } else {
+      const uint4 v2 = ldg16(g + 4);
+      u[4] = v2.x, u[5] = v2.y, u[6] = v2.z, u[7] = v2.w;
+      words_to_floats<float>(u, f);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = w && e + k >= 0 && e + k < K ? weight_at(w, w_bf16, e + k) : 1.f;
+  }
+}
+
+// four values to signed bytes (the conversion saturates)
+__device__ __forceinline__ uint32_t pack_s8(int a, int b, int c, int d) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\t"
+      "cvt.pack.sat.s8.s32.b32 t, %4, %3, 0;\n\t"
+      "cvt.pack.sat.s8.s32.b32 %0, %2, %1, t;\n\t}"
+      : "=r"(r)
+      : "r"(a), "r"(b), "r"(c), "r"(d));
+  return r;
+}
+
+// A row's bytes, 8 per vector, to q (which starts at a multiple of 8 where `vec`).  Skewed vectors
+// start `off` bytes before multiples of 8: they go through shared memory (`line`, 8 bytes per
+// vector and 8 more), where the 8 bytes from 8 j on are 8 of a vector and the next one.
+template <int VPT, int G, int LAYOUT>
+__device__ __forceinline__ void store_bytes(int8_t *q, uint2 (&b)[VPT], uint2 *line, int off, int tid, int size, int K,
+                                            bool vec) {
+  if constexpr (LAYOUT == kSkewed) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) line[i * size + tid] = b[i];
+    if constexpr (G == 32)
+      __syncwarp();
+    else
+      __syncthreads();
+    const int s = 8 * (off & 3);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const uint2 lo = line[i * size + tid], hi = line[i * size + tid + 1];
+      const uint32_t c0 = off & 4 ? lo.y : lo.x, c1 = off & 4 ? hi.x : lo.y, c2 = off & 4 ? hi.y : hi.x;
+      b[i] = make_uint2(__funnelshift_r(c0, c1, s), __funnelshift_r(c1, c2, s));
+    }
+    if constexpr (G == 32) __syncwarp();
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int e = (i * size + tid) * 8;
+    if (LAYOUT == kAligned ? e < K : vec && e + 8 <= K) {
+      *reinterpret_cast<uint2 *>(q + e) = b[i];
+    } else if (LAYOUT != kAligned) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (e + k < K) q[e + k] = (int8_t)((k < 4 ? b[i].x : b[i].y) >> (8 * (k & 3)));
+    }
+  }
+}
+
+// Over the group: a warp, or the whole block of at most G threads.
+template <int G>
+__device__ __forceinline__ float group_sum(float v, float *red) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (G > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int warps = blockDim.x >> 5;
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < G / 32; ++i)
+      if (i < warps) v += red[i];
+  }
+  return v;
+}
+template <int G>
+__device__ __forceinline__ uint32_t group_max(uint32_t v, uint32_t *red) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if constexpr (G > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int warps = blockDim.x >> 5;
+#pragma unroll
+    for (int i = 0; i < G / 32; ++i)
+      if (i < warps) v = max(v, red[i]);
+  }
+  return v;
+}
+
+constexpr int row_block(int G) { return G == 32 ? 256 : G; }  // (most) threads per block
+// threads of the group this thread belongs to
+template <int G>
+__device__ __forceinline__ int group_size() {
+  return G == 32 ? 32 : blockDim.x;
+}
+
+// What bounds it is the rows' one trip from and to HBM; see launch_width for the widths' groups
+// and what they measured.
+template <typename T, int MODE, int G, int VPT, int LAYOUT>
+__global__ void __launch_bounds__(row_block(G)) row_kernel(const RowArgs a) {
+  __shared__ float red_sum[2][32];
+  __shared__ uint32_t red_max[2][32];
+  constexpr int kPer = row_block(G) / G;  // rows of a block at a time
+  __shared__ uint2 line[LAYOUT == kSkewed && MODE != kNorm ? kPer * (G * VPT + 1) : 1];
+  constexpr bool kTwo = MODE != kQuantInt8;  // a second input: the residual, or SwiGLU's other half
+  constexpr bool kIsNorm = MODE == kNorm || MODE == kNormInt8;
+  const int size = group_size<G>(), tid = G == 32 ? threadIdx.x % 32 : threadIdx.x, K = a.K;
+  const long long first = (long long)blockIdx.x * kPer + (G == 32 ? threadIdx.x / 32 : 0);
+  const long long step = LAYOUT == kSkewed ? (long long)gridDim.x * kPer : a.rows;
+  const int off = LAYOUT == kSkewed ? misalign(static_cast<const T *>(a.x) + first * a.x_stride) : 0;
+  auto at = [&](int i) { return (i * size + tid) * 8 - off; };  // where the thread's i-th vector starts
+  float w[kIsNorm && LAYOUT == kSkewed ? VPT * 8 : 1];
+  if constexpr (kIsNorm && LAYOUT == kSkewed) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) weights8(a.w, a.w_bf16, false, at(i), K, w + 8 * i);
+  }
+  // the tensors' extents
+  const T *x_begin = static_cast<const T *>(a.x), *x_end = x_begin + (a.rows - 1) * a.x_stride + (MODE == kSwigluInt8 ? 2 : 1) * (long long)K;
+  const T *r_begin = MODE == kSwigluInt8 ? x_begin : static_cast<const T *>(a.r);
+  const T *r_end = MODE == kSwigluInt8 ? x_end : r_begin + (a.rows - 1) * a.r_stride + K;
+  int flip = 0;
+  // (where a group is a block, the block's threads leave the loop together; else whole warps do)
+  for (long long row = first; row < a.rows; row += step) {
+    const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+    const T *r = MODE == kSwigluInt8 ? x + K : a.r ? static_cast<const T *>(a.r) + row * a.r_stride : nullptr;
+    float v[VPT * 8];
+    {
+      Vec8<T, LAYOUT> vx[VPT], vr[VPT];
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) vx[i].load(x, at(i), K, x_begin, x_end);
+      if (kTwo && r) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) vr[i].load(r, at(i), K, r_begin, r_end);
+      }
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float *f = v + 8 * i;
+        vx[i].unpack(f, at(i), K);
+        if (kTwo && r) {
+          float g[8];
+          vr[i].unpack(g, at(i), K);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = MODE == kSwigluInt8 ? silu_mul(f[j], g[j]) : to_f<T>(from_f<T>(f[j] + g[j]));
+          if (MODE != kSwigluInt8) store8<T, LAYOUT>(static_cast<T *>(a.h) + row * K, at(i), K, f);
+        }
+      }
+    }
+
+    if constexpr (kIsNorm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < VPT * 8; ++i) ss = fmaf(v[i], v[i], ss);
+      const float rstd = rsqrtf(group_sum<G>(ss, red_sum[flip]) / (float)K + a.eps);
+      if (a.rstd && tid == 0) a.rstd[row] = rstd;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float u[8];
+        if (LAYOUT != kSkewed) weights8(a.w, a.w_bf16, LAYOUT == kAligned && at(i) < K, at(i), K, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[8 * i + j] = v[8 * i + j] * rstd * (LAYOUT == kSkewed ? w[kIsNorm && LAYOUT == kSkewed ? 8 * i + j : 0] : u[j]);
+      }
+    }
+    if constexpr (MODE == kNorm) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) store8<T, LAYOUT>(static_cast<T *>(a.y) + row * K, at(i), K, v + 8 * i);
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < VPT * 8; ++i) m = max(m, abs_bits(v[i]));  // (0 past a row's ends)
+      const Quantiser qz(group_max<G>(m, red_max[flip]));
+      if (tid == 0) a.scale[row] = qz.scale;
+      if (qz.lift != 1.f) {
+#pragma unroll
+        for (int i = 0; i < VPT * 8; ++i) v[i] *= qz.lift;
+      }
+      int8_t *q = a.q + row * a.q_stride;
+      uint2 b[VPT];
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const float *f = v + 8 * i;
+        b[i] = make_uint2(pack_s8(qz(f[0]), qz(f[1]), qz(f[2]), qz(f[3])), pack_s8(qz(f[4]), qz(f[5]), qz(f[6]), qz(f[7])));
+      }
+      store_bytes<VPT, G, LAYOUT>(q, b, line + (threadIdx.x / 32) * (G == 32 ? VPT * 32 + 1 : 0), off, tid, size, K, a.q_vec);
+    }
+    flip ^= 1;  // the next row's barrier lies between two uses of a half
+  }
+}
 
 // Any width: the row is read again for each of its passes (from the caches).
 template <typename T, int MODE>
@@ -135,7 +495,7 @@ __global__ void __launch_bounds__(kNT) row_loop_kernel(RowArgs a) {
   if (threadIdx.x == 0) a.scale[row] = qz.scale;
   int8_t *q = a.q + row * a.q_stride;
   for (int i = threadIdx.x; i < K; i += kNT) {
-    q[i] = (int8_t)qz(value(i));
+    q[i] = (int8_t)qz(value(i) * qz.lift);
     if (MODE == kNormInt8 && r) h[i] = from_f<T>(stream(i));
   }
 }
@@ -178,22 +538,119 @@ __global__ void __launch_bounds__(kNT) bwd_loop_kernel(BwdArgs a) {
   }
 }
 
-// dw[k] = sum of the blocks' partial sums, in their order.
-__global__ void __launch_bounds__(256) dw_sum_kernel(const float *part, int n, int K, void *dw, int w_bf16) {
-  __shared__ float red[8][32];
-  const int k = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+// A group of G threads walks rows; a thread keeps its columns' weights and sums of dw in
+// registers over all of them, and where the group is a block (whose barrier every row pays) it
+// has the next row's values on their way while it works on this one's.
+template <typename T, int G, int VPT, int LAYOUT>
+__global__ void __launch_bounds__(row_block(G), G <= 256 ? 2 : 1) bwd_kernel(const BwdArgs a) {
+  constexpr int kPer = row_block(G) / G, N = VPT * 8;
+  constexpr bool kAhead = G > 32;
+  __shared__ float red[2][32];
+  extern __shared__ float warp_dw[];  // [groups of the block][K], where a block has several
+  const int size = group_size<G>(), tid = G == 32 ? threadIdx.x % 32 : threadIdx.x, K = a.K;
+  const int group = blockIdx.x * kPer + (G == 32 ? threadIdx.x / 32 : 0), groups = gridDim.x * kPer;
+  const int off = LAYOUT == kSkewed ? misalign(static_cast<const T *>(a.dy) + (long long)group * K) : 0;
+  auto at = [&](int i) { return (i * size + tid) * 8 - off; };  // where the thread's i-th vector starts
+  float w[N], acc[N];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) weights8(a.w, a.w_bf16, false, at(i), K, w + 8 * i);
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+
+  struct Row {
+    Vec8<T, LAYOUT> dy[VPT], h[VPT], dh[VPT];
+    float rstd;
+  };
+  auto load = [&](Row &s, long long row) {
+    const T *dy = static_cast<const T *>(a.dy) + row * K, *h = static_cast<const T *>(a.h) + row * K;
+    const T *dh = a.dh ? static_cast<const T *>(a.dh) + row * K : nullptr;
+    s.rstd = __ldg(a.rstd + row);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      s.dy[i].load(dy, at(i), K, dy - row * K, dy + (a.rows - row) * K);
+      s.h[i].load(h, at(i), K, h - row * K, h + (a.rows - row) * K);
+      if (dh) s.dh[i].load(dh, at(i), K, dh - row * K, dh + (a.rows - row) * K);
+    }
+  };
+  int flip = 0;
+  Row s;
+  if (kAhead && group < a.rows) load(s, group);
+  for (long long row = group; row < a.rows; row += groups) {
+    Row next;
+    if (kAhead) {
+      if (row + groups < a.rows) load(next, row + groups);
+    } else {
+      load(s, row);
+    }
+    const float rstd = s.rstd;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float y[8], x[8];
+      s.dy[i].unpack(y, at(i), K);
+      s.h[i].unpack(x, at(i), K);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = fmaf(y[j] * w[8 * i + j], x[j], sum);
+    }
+    const float c = group_sum<G>(sum, red[flip]) * rstd * rstd / (float)K;
+    T *dx = static_cast<T *>(a.dx) + row * K;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float y[8], x[8], d[8];
+      s.dy[i].unpack(y, at(i), K);
+      s.h[i].unpack(x, at(i), K);
+      if (a.dh) s.dh[i].unpack(d, at(i), K);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        acc[8 * i + j] = fmaf(y[j], x[j] * rstd, acc[8 * i + j]);
+        y[j] = rstd * fmaf(y[j], w[8 * i + j], -x[j] * c);
+        if (a.dh) y[j] += d[j];
+      }
+      store8<T, LAYOUT>(dx, at(i), K, y);
+    }
+    flip ^= 1;  // a barrier of the next row lies between two uses of a half
+    if (kAhead) s = next;
+  }
+  if (!a.part) return;
+  float *part = a.part + (long long)blockIdx.x * K;
+  float *mine = kPer == 1 ? part : warp_dw + (threadIdx.x / 32) * K;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (at(i) + j >= 0 && at(i) + j < K) mine[at(i) + j] = acc[8 * i + j];
+  if constexpr (kPer > 1) {
+    __syncthreads();
+    for (int c = threadIdx.x; c < K; c += row_block(G)) {
+      float v = 0.f;
+#pragma unroll
+      for (int g = 0; g < kPer; ++g) v += warp_dw[g * K + c];
+      part[c] = v;
+    }
+  }
+}
+
+// dw[k] = sum of the blocks' partial sums, in a fixed order.
+__global__ void __launch_bounds__(1024) dw_sum_kernel(const float *part, int n, int K, void *dw, int w_bf16) {
+  __shared__ float red[32][33];
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, k = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (k < K)
-    for (int i = g; i < n; i += 8) s += part[(long long)i * K + k];
-  red[g][threadIdx.x & 31] = s;
+  if (k < K) {
+#pragma unroll 4
+    for (int i = g; i < n; i += 32) s += part[(long long)i * K + k];
+  }
+  red[g][lane] = s;
   __syncthreads();
-  if (g == 0 && k < K) {
-    s = 0.f;
-    for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
+  // transposed: warp g adds column g
+  s = red[lane][g];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int c = blockIdx.x * 32 + g;
+  if (lane == 0 && c < K) {
     if (w_bf16)
-      static_cast<__nv_bfloat16 *>(dw)[k] = __float2bfloat16_rn(s);
+      static_cast<__nv_bfloat16 *>(dw)[c] = __float2bfloat16_rn(s);
     else
-      static_cast<float *>(dw)[k] = s;
+      static_cast<float *>(dw)[c] = s;
   }
 }
 
@@ -207,7 +664,7 @@ __global__ void __launch_bounds__(256) dequant_kernel(const int8_t *q, long long
 }
 
 // ------------------------------------------------------------------ host side
-int check_rows(const char *what, int64_t rows, int64_t K, int dtype) {
+int check_rows(const char *what, int64_t rows, int64_t K, int dtype, std::initializer_list<const void *> values = {}) {
   char buf[160];
   if (dtype != RACE_F32 && dtype != RACE_BF16) {
     snprintf(buf, sizeof(buf), "%s: dtype %d", what, dtype);
@@ -218,20 +675,133 @@ int check_rows(const char *what, int64_t rows, int64_t K, int dtype) {
     snprintf(buf, sizeof(buf), "%s: rows=%lld (1..2^31-1), width=%lld (1..2^24)", what, (long long)rows, (long long)K);
     return race::report_error(RACE_ERR_SHAPE, buf);
   }
+  for (const void *p : values)
+    if (reinterpret_cast<uintptr_t>(p) % (dtype == RACE_F32 ? 4 : 2)) {
+      snprintf(buf, sizeof(buf), "%s: a tensor does not start at a multiple of its values' size", what);
+      return race::report_error(RACE_ERR_ALIGN, buf);
+    }
   return RACE_OK;
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Threads that `vectors` vectors at VPT per thread want: whole warps.
+int threads_for(int vectors, int VPT) { return (vectors + 32 * VPT - 1) / (32 * VPT) * 32; }
+
+template <typename T, int MODE, int G, int VPT, int LAYOUT>
+void launch_row_kernel(const RowArgs &a, int vectors, cudaStream_t s) {
+  constexpr int kPer = row_block(G) / G;
+  const int threads = G == 32 ? row_block(G) : threads_for(vectors, VPT);
+  long long blocks = (a.rows + kPer - 1) / kPer;
+  if (LAYOUT == kSkewed) {
+    // groups that walk rows, a multiple of 8 of them: as many as an SM's 2048 threads hold
+    const long long most = 148 * (2048 / threads) / 8 * 8;
+    blocks = blocks < most ? (blocks + 7) / 8 * 8 : most;
+  }
+  row_kernel<T, MODE, G, VPT, LAYOUT><<<(unsigned)blocks, threads, 0, s>>>(a);
+}
+
+// Threads per row.  A warp up to 1024 values: no barriers, all of a row's loads in flight at
+// once.  Wider rows take a block with two vectors per thread (32768 x 2048 bf16: norm 80 us with
+// 128 threads, 83 with 64, 124 with a warp; 8-bit norm 70, 83, 132), four past 4096 values (8192:
+// norm 159 us with 256 threads, 171 with 512, 198 with 1024) except in the 8-bit norm, whose
+// registers then leave too few blocks per SM (183 us with 256, 147 with 512).  Few rows spread
+// each over more threads, for latency.
+template <typename T, int MODE, int LAYOUT>
+void launch_width(const RowArgs &a, cudaStream_t s) {
+  const int n = (a.K + (LAYOUT == kSkewed ? 7 : 0) + 7) / 8;  // vectors, whatever the offset
+  const bool few = a.rows < 1184;  // eight blocks on each SM of a B200
+  if (n <= 32) return launch_row_kernel<T, MODE, 32, 1, LAYOUT>(a, n, s);
+  if (n <= 256 && few) return launch_row_kernel<T, MODE, 256, 1, LAYOUT>(a, n, s);
+  if (n <= 64) return launch_row_kernel<T, MODE, 32, 2, LAYOUT>(a, n, s);
+  if (n <= 96) return launch_row_kernel<T, MODE, 32, 3, LAYOUT>(a, n, s);
+  if (n <= 128) return launch_row_kernel<T, MODE, 32, 4, LAYOUT>(a, n, s);
+  if (n <= 576) return launch_row_kernel<T, MODE, 288, 2, LAYOUT>(a, n, s);
+  if (n <= 1152 && (few || MODE == kNormInt8)) return launch_row_kernel<T, MODE, 576, 2, LAYOUT>(a, n, s);
+  if (n <= 1152) return launch_row_kernel<T, MODE, 288, 4, LAYOUT>(a, n, s);
+  if (n <= 2048) return launch_row_kernel<T, MODE, 1024, 2, LAYOUT>(a, n, s);
+  if constexpr (LAYOUT == kAligned) {
+    if (n <= 4096) return launch_row_kernel<T, MODE, 1024, 4, LAYOUT>(a, n, s);
+  }
+  row_loop_kernel<T, MODE><<<(unsigned)a.rows, kNT, 0, s>>>(a);
+}
+
+// How far past a multiple of 16 bytes.
+int past16(const void *p, int64_t bytes = 0) { return (int)((reinterpret_cast<uintptr_t>(p) + (uint64_t)bytes) & 15); }
+
+template <typename T, int MODE>
+void launch_type(RowArgs a, cudaStream_t s) {
+  const int64_t size = sizeof(T);
+  a.q_vec = (reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)a.q_stride) % 8 == 0;
+  if constexpr (MODE == kSwigluInt8) {
+    if (a.K % 8 == 0 && aligned16(a.x) && past16(nullptr, a.x_stride * size) == 0 && a.q_vec)
+      launch_width<T, MODE, kAligned>(a, s);
+    else
+      launch_width<T, MODE, kShifted>(a, s);
+  } else {
+    // whether the tensors' rows all start equally far into a granule: the first, and the step
+    const int base = past16(a.x), step = past16(nullptr, a.x_stride * size), dense = past16(nullptr, a.K * size);
+    bool alike = (!a.r || (past16(a.r) == base && past16(nullptr, a.r_stride * size) == step)) &&
+                 (!(a.r || a.y) || dense == step) && (!a.y || past16(a.y) == base) && (!a.r || past16(a.h) == base);
+    if (alike && base == 0 && step == 0 && a.K % 8 == 0 && aligned16(a.w) && a.q_vec)
+      launch_width<T, MODE, kAligned>(a, s);
+    else if (alike)
+      launch_width<T, MODE, kSkewed>(a, s);
+    else  // a view beside dense tensors, say
+      row_loop_kernel<T, MODE><<<(unsigned)a.rows, kNT, 0, s>>>(a);
+  }
 }
 
 template <int MODE>
 int launch_rows(const char *what, const RowArgs &a, int dtype, cudaStream_t s) {
   if (dtype == RACE_BF16)
-    row_loop_kernel<__nv_bfloat16, MODE><<<(unsigned)a.rows, kNT, 0, s>>>(a);
+    launch_type<__nv_bfloat16, MODE>(a, s);
   else
-    row_loop_kernel<float, MODE><<<(unsigned)a.rows, kNT, 0, s>>>(a);
+    launch_type<float, MODE>(a, s);
   return launched(what);
 }
 
-// blocks of the backward: each keeps one row of partial sums of dw
-int bwd_blocks(int64_t rows) { return (int)(rows < 1184 ? rows : 1184); }
+// Blocks of the backward, each with one row of partial sums of dw to be added: four per SM of
+// a B200, or fewer with a row or two each.  A multiple of 8 (see kSkewed).
+constexpr int kBwdBlocks = 592;
+int bwd_blocks(int64_t rows, int64_t K) {
+  const int64_t n = K <= 768 ? (rows + 1) / 2 : rows;
+  return (int)(n < kBwdBlocks ? (n + 7) / 8 * 8 : kBwdBlocks);
+}
+
+template <typename T, int G, int VPT, int LAYOUT>
+void launch_bwd_kernel(const BwdArgs &a, int blocks, int vectors, cudaStream_t s) {
+  constexpr int kPer = row_block(G) / G;
+  const int threads = G == 32 ? row_block(G) : threads_for(vectors, VPT);
+  const size_t smem = a.part && kPer > 1 ? sizeof(float) * kPer * (size_t)a.K : 0;  // at most 24 KB
+  bwd_kernel<T, G, VPT, LAYOUT><<<blocks, threads, smem, s>>>(a);
+}
+
+template <typename T, int LAYOUT>
+void launch_bwd_width(const BwdArgs &a, int blocks, cudaStream_t s) {
+  const int n = (a.K + (LAYOUT == kSkewed ? 7 : 0) + 7) / 8;
+  if (n <= 32) return launch_bwd_kernel<T, 32, 1, LAYOUT>(a, blocks, n, s);
+  if (n <= 64) return launch_bwd_kernel<T, 32, 2, LAYOUT>(a, blocks, n, s);
+  if (n <= 96) return launch_bwd_kernel<T, 32, 3, LAYOUT>(a, blocks, n, s);
+  if (n <= 128) return launch_bwd_kernel<T, 128, 1, LAYOUT>(a, blocks, n, s);
+  if (n <= 256) return launch_bwd_kernel<T, 256, 1, LAYOUT>(a, blocks, n, s);
+  if (n <= 512) return launch_bwd_kernel<T, 512, 1, LAYOUT>(a, blocks, n, s);
+  if (n <= 1024) return launch_bwd_kernel<T, 512, 2, LAYOUT>(a, blocks, n, s);
+  if (n <= 2048) return launch_bwd_kernel<T, 512, 4, LAYOUT>(a, blocks, n, s);
+  bwd_loop_kernel<T><<<blocks, kNT, 0, s>>>(a);
+}
+
+template <typename T>
+void launch_bwd(const BwdArgs &a, int blocks, cudaStream_t s) {
+  const int base = past16(a.dy);
+  const bool alike = past16(a.h) == base && past16(a.dx) == base && (!a.dh || past16(a.dh) == base);
+  if (alike && base == 0 && a.K % 8 == 0)
+    launch_bwd_width<T, kAligned>(a, blocks, s);
+  else if (alike)
+    launch_bwd_width<T, kSkewed>(a, blocks, s);
+  else
+    bwd_loop_kernel<T><<<blocks, kNT, 0, s>>>(a);
+}
 
 }  // namespace
 
@@ -241,7 +811,7 @@ int race_rms_norm_fwd(const void *x, int64_t x_stride, const void *residual, int
                       const void *weight, int weight_dtype, void *y, void *h, float *rstd, int64_t rows, int64_t K,
                       float eps, void *stream) {
   if (!x || !y || (residual && !h)) return err(RACE_ERR_ARG, "race_rms_norm_fwd: null pointer");
-  if (const int rc = check_rows("race_rms_norm_fwd", rows, K, dtype)) return rc;
+  if (const int rc = check_rows("race_rms_norm_fwd", rows, K, dtype, {x, residual, y, h})) return rc;
   if (weight && weight_dtype != RACE_F32 && weight_dtype != RACE_BF16)
     return err(RACE_ERR_DTYPE, "race_rms_norm_fwd: weight dtype %lld", weight_dtype);
   if (x_stride < K || (residual && residual_stride < K)) return err(RACE_ERR_SHAPE, "race_rms_norm_fwd: row stride below the width %lld", K);
@@ -253,7 +823,7 @@ int race_rms_norm_int8(const void *x, int64_t x_stride, const void *residual, in
                        const void *weight, int weight_dtype, int8_t *q, int64_t q_stride, float *scale, void *h,
                        int64_t rows, int64_t K, float eps, void *stream) {
   if (!x || !q || !scale || (residual && !h)) return err(RACE_ERR_ARG, "race_rms_norm_int8: null pointer");
-  if (const int rc = check_rows("race_rms_norm_int8", rows, K, dtype)) return rc;
+  if (const int rc = check_rows("race_rms_norm_int8", rows, K, dtype, {x, residual, h})) return rc;
   if (weight && weight_dtype != RACE_F32 && weight_dtype != RACE_BF16)
     return err(RACE_ERR_DTYPE, "race_rms_norm_int8: weight dtype %lld", weight_dtype);
   if (x_stride < K || q_stride < K || (residual && residual_stride < K))
@@ -265,7 +835,7 @@ int race_rms_norm_int8(const void *x, int64_t x_stride, const void *residual, in
 int race_quant_int8(const void *x, int64_t x_stride, int dtype, int8_t *q, int64_t q_stride, float *scale, int64_t rows,
                     int64_t K, void *stream) {
   if (!x || !q || !scale) return err(RACE_ERR_ARG, "race_quant_int8: null pointer");
-  if (const int rc = check_rows("race_quant_int8", rows, K, dtype)) return rc;
+  if (const int rc = check_rows("race_quant_int8", rows, K, dtype, {x})) return rc;
   if (x_stride < K || q_stride < K) return err(RACE_ERR_SHAPE, "race_quant_int8: row stride below the width %lld", K);
   RowArgs a{x, nullptr, nullptr, nullptr, nullptr, q, scale, nullptr, rows, x_stride, 0, q_stride, (int)K, 0, 0.f};
   return launch_rows<kQuantInt8>("quant_int8", a, dtype, reinterpret_cast<cudaStream_t>(stream));
@@ -274,7 +844,7 @@ int race_quant_int8(const void *x, int64_t x_stride, int dtype, int8_t *q, int64
 int race_swiglu_int8(const void *gate_up, int64_t stride, int dtype, int8_t *q, int64_t q_stride, float *scale,
                      int64_t rows, int64_t F, void *stream) {
   if (!gate_up || !q || !scale) return err(RACE_ERR_ARG, "race_swiglu_int8: null pointer");
-  if (const int rc = check_rows("race_swiglu_int8", rows, F, dtype)) return rc;
+  if (const int rc = check_rows("race_swiglu_int8", rows, F, dtype, {gate_up})) return rc;
   if (stride < 2 * F || q_stride < F) return err(RACE_ERR_SHAPE, "race_swiglu_int8: row stride below the width (F=%lld)", F);
   RowArgs a{gate_up, nullptr, nullptr, nullptr, nullptr, q, scale, nullptr, rows, stride, 0, q_stride, (int)F, 0, 0.f};
   return launch_rows<kSwigluInt8>("swiglu_int8", a, dtype, reinterpret_cast<cudaStream_t>(stream));
@@ -296,28 +866,28 @@ int race_dequant_int8(const int8_t *q, int64_t q_stride, const float *scale, voi
 
 size_t race_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t K) {
   if (rows < 1 || K < 1) return 0;
-  return sizeof(float) * (size_t)bwd_blocks(rows) * (size_t)K;
+  return sizeof(float) * (size_t)bwd_blocks(rows, K) * (size_t)K;
 }
 
 int race_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float *rstd, int dtype, const void *weight,
                       int weight_dtype, void *dx, void *dw, int64_t rows, int64_t K, void *workspace,
                       size_t workspace_bytes, void *stream) {
   if (!dy || !h || !rstd || !dx) return err(RACE_ERR_ARG, "race_rms_norm_bwd: null pointer");
-  if (const int rc = check_rows("race_rms_norm_bwd", rows, K, dtype)) return rc;
+  if (const int rc = check_rows("race_rms_norm_bwd", rows, K, dtype, {dy, dh, h, dx})) return rc;
   if ((weight || dw) && weight_dtype != RACE_F32 && weight_dtype != RACE_BF16)
     return err(RACE_ERR_DTYPE, "race_rms_norm_bwd: weight dtype %lld", weight_dtype);
   if (dw && (!workspace || workspace_bytes < race_rms_norm_bwd_workspace_bytes(rows, K)))
     return err(RACE_ERR_WORKSPACE, "race_rms_norm_bwd: workspace of %lld bytes needed", (long long)race_rms_norm_bwd_workspace_bytes(rows, K));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int blocks = bwd_blocks(rows);
+  const int blocks = bwd_blocks(rows, K);
   BwdArgs a{dy, dh, h, weight, rstd, dx, dw, dw ? static_cast<float *>(workspace) : nullptr, rows, (int)K, weight_dtype == RACE_BF16};
   if (dtype == RACE_BF16)
-    bwd_loop_kernel<__nv_bfloat16><<<blocks, kNT, 0, s>>>(a);
+    launch_bwd<__nv_bfloat16>(a, blocks, s);
   else
-    bwd_loop_kernel<float><<<blocks, kNT, 0, s>>>(a);
+    launch_bwd<float>(a, blocks, s);
   if (const int rc = launched("rms_norm_bwd")) return rc;
   if (!dw) return RACE_OK;
-  dw_sum_kernel<<<(unsigned)((K + 31) / 32), 256, 0, s>>>(a.part, blocks, (int)K, dw, weight_dtype == RACE_BF16);
+  dw_sum_kernel<<<(unsigned)((K + 31) / 32), 1024, 0, s>>>(a.part, blocks, (int)K, dw, weight_dtype == RACE_BF16);
   return launched("rms_norm_bwd dw");
 }
 
