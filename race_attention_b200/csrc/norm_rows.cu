@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(kNT) bwd_loop_kernel(BwdArgs a) {
 // registers over all of them, and where the group is a block (whose barrier every row pays) it
 // has the next row's values on their way while it works on this one's.
 template <typename T, int G, int VPT, int LAYOUT>
-__global__ void __launch_bounds__(row_block(G), G <= 256 ? 2 : 1) bwd_kernel(const BwdArgs a) {
+__global__ void __launch_bounds__(row_block(G), G == 320 ? 2 : 512 / row_block(G)) bwd_kernel(const BwdArgs a) {
   constexpr int kPer = row_block(G) / G, N = VPT * 8;
   constexpr bool kAhead = G > 32;
   __shared__ float red[2][32];
@@ -762,11 +762,11 @@ int launch_rows(const char *what, const RowArgs &a, int dtype, cudaStream_t s) {
 }
 
 // Blocks of the backward, each with one row of partial sums of dw to be added: four per SM of
-// a B200, or fewer with a row or two each.  A multiple of 8 (see kSkewed).
-constexpr int kBwdBlocks = 592;
+// a B200, eight where they are of 64 threads; with few rows a row each, then four (in a warp
+// of its own each up to 768 values).  A multiple of 8 (see kSkewed).
 int bwd_blocks(int64_t rows, int64_t K) {
-  const int64_t n = K <= 768 ? (rows + 1) / 2 : rows;
-  return (int)(n < kBwdBlocks ? (n + 7) / 8 * 8 : kBwdBlocks);
+  const int64_t n = rows <= 148 ? rows : rows <= 592 ? 148 : (rows + 3) / 4, most = K > 768 && K <= 1024 ? 1184 : 592;
+  return (int)(n < most ? (n + 7) / 8 * 8 : most);
 }
 
 template <typename T, int G, int VPT, int LAYOUT>
@@ -783,8 +783,18 @@ void launch_bwd_width(const BwdArgs &a, int blocks, cudaStream_t s) {
   if (n <= 32) return launch_bwd_kernel<T, 32, 1, LAYOUT>(a, blocks, n, s);
   if (n <= 64) return launch_bwd_kernel<T, 32, 2, LAYOUT>(a, blocks, n, s);
   if (n <= 96) return launch_bwd_kernel<T, 32, 3, LAYOUT>(a, blocks, n, s);
+  // Two vectors per thread keep more bytes on their way (bf16, aligned: 65536 x 1024 101 us
+  // against 134, 32768 x 2048 105 against 149); with fp32 or skewed rows they cost registers
+  // that the blocks then lack (fp32 32768 x 2048 237 us against 168, bf16 65536 x 1001 196
+  // against 138).
+  if constexpr (sizeof(T) == 2 && LAYOUT == kAligned) {
+    if (n <= 128) return launch_bwd_kernel<T, 64, 2, LAYOUT>(a, blocks, n, s);
+    if (n <= 256) return launch_bwd_kernel<T, 128, 2, LAYOUT>(a, blocks, n, s);
+    if (n <= 512) return launch_bwd_kernel<T, 256, 2, LAYOUT>(a, blocks, n, s);
+  }
   if (n <= 128) return launch_bwd_kernel<T, 128, 1, LAYOUT>(a, blocks, n, s);
   if (n <= 256) return launch_bwd_kernel<T, 256, 1, LAYOUT>(a, blocks, n, s);
+  if (n <= 320) return launch_bwd_kernel<T, 320, 1, LAYOUT>(a, blocks, n, s);
   if (n <= 512) return launch_bwd_kernel<T, 512, 1, LAYOUT>(a, blocks, n, s);
   if (n <= 1024) return launch_bwd_kernel<T, 512, 2, LAYOUT>(a, blocks, n, s);
   if (n <= 2048) return launch_bwd_kernel<T, 512, 4, LAYOUT>(a, blocks, n, s);
