@@ -18,7 +18,7 @@
 // The forward reads a row once, by a block or (few rows) a cluster of up to 8 blocks with a
 // share each: every thread keeps its running maximum, S and U, and where its maximum lies, and
 // the threads' are joined at the end.  The alternatives need no second pass over the row: the
-// n-th largest of the threads' maxima (in fact of groups of 8 threads) bounds the n-th largest
+// n-th largest of the threads' maxima (or of groups of four threads) bounds the n-th largest
 // entry from below, and only the few threads whose maximum reaches it hold candidates, whose
 // entries are read again from the L2 cache.
 #include "race_b200.h"
@@ -35,12 +35,8 @@ using race::from_f;
 using race::launched;
 using race::to_f;
 
-constexpr int kNT = 512;
-constexpr int kWarps = kNT / 32;
 constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 8;
-constexpr int kGroup = 8;               // threads whose joint maximum enters the bound
-constexpr int kCandidates = 1024;       // entries at or above the bound that are ranked at once
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct FwdArgs {
@@ -169,18 +165,19 @@ struct Stat {
     s *= k;
     m = to;
   }
-  __device__ __forceinline__ void join(const Stat &o, float c) {
-    Stat p = o;
-    const float to = fmaxf(m, o.m);
+  // those of the whole warp, in every lane
+  __device__ __forceinline__ void join_warp(float c) {
+    float to = m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, o));
     rebase(to, c);
-    p.rebase(to, c);
-    s += p.s;
-    u += p.u;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      u += __shfl_xor_sync(0xffffffffu, u, o);
+    }
   }
 };
-__device__ __forceinline__ Stat shfl_xor(const Stat &v, int o) {
-  return {__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o), __shfl_xor_sync(0xffffffffu, v.u, o)};
-}
 
 // ---- clusters
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -199,13 +196,14 @@ struct Shared {
 };
 
 // Grid: C blocks (a cluster) per row; block `rank` of a row takes its granules [G rank / C,
-// G (rank + 1) / C), thread t those at t, t + 512, ... of them, kBatch on their way at a time.
-template <typename T>
+// G (rank + 1) / C), thread t those at t, t + kNT, ... of them, kBatch on their way at a time.
+template <typename T, int kNT>
 __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, const int C) {
-  constexpr int kBatch = 4;
+  constexpr int kBatch = 4, kWarps = kNT / 32;
+  constexpr int kCandidates = kNT == 32 ? 256 : 1024;  // entries at or above the bound that are ranked at once
   __shared__ Shared sh;
   __shared__ Stat warp_stat[kWarps];
-  __shared__ unsigned long long bound[kNT / kGroup], cand[kCandidates], tau;
+  __shared__ unsigned long long bound[kNT], cand[kCandidates], tau;
   __shared__ int n_owner, n_cand, owner[kNT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = blockIdx.x % C;
@@ -271,36 +269,39 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
     st.u += u2.x + u2.y;
   }
   const float thread_max = st.m;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) st.join(shfl_xor(st, o), a.c);
+  st.join_warp(a.c);
   if (lane == 0) warp_stat[warp] = st;
 
   // ---- alternatives of this block's share: candidates are what reaches tau
   const bool top = a.n_top > 0;
   unsigned long long mine = 0;  // 0: no entries
+  // threads whose joint maximum enters the bound: four where that leaves more than 32 of them
+  // with entries (fewer keys to rank), else one
+  constexpr int kGroup = kNT >= 256 ? 4 : 1;
+  const int group = g1 - g0 >= kNT ? kGroup : 1, n_keys = kNT / group;
   if (top) {
     // upper end of the granule: an index no lower than the first maximum's
     if (g0 + tid < g1) mine = order_key(thread_max, view.first(best) + kPer<T> - 1);
     unsigned long long k = mine;
-#pragma unroll
-    for (int o = 1; o < kGroup; o <<= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
-    if (lane % kGroup == 0) bound[tid / kGroup] = k;
+    if (group == 4) {
+      k = max(k, __shfl_xor_sync(0xffffffffu, k, 1));
+      k = max(k, __shfl_xor_sync(0xffffffffu, k, 2));
+    }
+    if (tid % group == 0) bound[tid / group] = k;
     if (tid == 0) n_owner = n_cand = 0, tau = 0;
   }
   __syncthreads();
   if (warp == 0) {
-    Stat b = lane < kWarps ? warp_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
-#pragma unroll
-    for (int o = kWarps / 2; o; o >>= 1) b.join(shfl_xor(b, o), a.c);
-    if (lane == 0) sh.stat[rank] = b;
-    st = b;
+    st = lane < kWarps ? warp_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
+    st.join_warp(a.c);
+    if (lane == 0) sh.stat[rank] = st;
   }
   if (top) {
-    if (tid < kNT / kGroup) {
+    if (tid < n_keys) {
       const unsigned long long k = bound[tid];
       int above = 0;
 #pragma unroll 8
-      for (int i = 0; i < kNT / kGroup; ++i) above += bound[i] > k;
+      for (int i = 0; i < n_keys; ++i) above += bound[i] > k;
       if (k && above == a.n_top - 1) tau = k;  // (keys of groups with entries differ)
     }
     __syncthreads();
@@ -391,14 +392,11 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
   if (C == 1 && !top && warp) return;
 
   // ---- the row's results
-  Stat all = lane < C ? sh.stat[lane] : Stat{-INFINITY, 0.f, 0.f};
-  if (C == 1 && !top) all = st;  // (warp 0, whose lanes all hold it)
-  else
-#pragma unroll
-    for (int o = kMaxCluster / 2; o; o >>= 1) all.join(shfl_xor(all, o), a.c);
-  all.m = __shfl_sync(0xffffffffu, all.m, 0);
-  all.s = __shfl_sync(0xffffffffu, all.s, 0);
-  all.u = __shfl_sync(0xffffffffu, all.u, 0);
+  Stat all = st;  // (in warp 0, the only one with C == 1 and no alternatives, every lane's)
+  if (C > 1 || top) {
+    all = lane < C ? sh.stat[lane] : Stat{-INFINITY, 0.f, 0.f};
+    all.join_warp(a.c);
+  }
   const bool empty = all.s == 0.f;
   const float lm = all.m == -INFINITY ? 0.f : all.m, log_s = empty ? -INFINITY : log2f(all.s);
   auto log_p = [&](float l) { return empty ? -INFINITY : (l - lm) * a.inv_temp - log_s * kLn2; };
@@ -454,9 +452,9 @@ struct RowGrad {
 
 // Rows of logits and gradient that start equally far into a granule (dense ones do): 16-byte
 // accesses but at a row's ends.  Grid (rows, shares of a row).
-template <typename T, bool ENTROPY>
+template <typename T, bool ENTROPY, int kNT>
 __global__ void __launch_bounds__(kNT) logprobs_bwd_kernel(const BwdArgs a) {
-  constexpr int kBatch = 2;
+  constexpr int kBatch = 2;  // (four leave room for fewer blocks: 8192 x 50257 bf16 343 us against 313)
   const long long row = blockIdx.x;
   const RowGrad g(a, row);
   const RowView<T> view(a.logits, row, a.stride, a.rows, a.V);
@@ -528,7 +526,7 @@ __global__ void __launch_bounds__(kNT) logprobs_bwd_kernel(const BwdArgs a) {
 }
 
 // Any layout, one value at a time.
-template <typename T>
+template <typename T, int kNT>
 __global__ void __launch_bounds__(kNT) logprobs_bwd_loop_kernel(const BwdArgs a) {
   const long long row = blockIdx.x;
   const RowGrad g(a, row);
@@ -545,12 +543,13 @@ __global__ void __launch_bounds__(kNT) logprobs_bwd_loop_kernel(const BwdArgs a)
   }
 }
 
-template <typename T>
-int launch_fwd(const FwdArgs &a, cudaStream_t s) {
+template <typename T, int kNT>
+int launch_fwd_threads(const FwdArgs &a, cudaStream_t s) {
   // Blocks per row: more while there are fewer than four blocks on each SM of a B200 and every
   // thread still has a granule.
   int C = 1;
-  while (C < kMaxCluster && a.rows * C * 2 <= 4 * 148 && a.V >= 2 * C * kNT * kPer<T>) C *= 2;
+  if (kNT == 256)
+    while (C < kMaxCluster && a.rows * C * 2 <= 4 * 148 && a.V >= 2 * C * kNT * kPer<T>) C *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * C));
   cfg.blockDim = dim3(kNT);
@@ -561,27 +560,42 @@ int launch_fwd(const FwdArgs &a, cudaStream_t s) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = C > 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T>, a, C);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, kNT>, a, C);
   if (e != cudaSuccess) return race::cuda_err("token_logprobs_fwd", e);
   return launched("token_logprobs_fwd");
 }
 
 template <typename T>
-int launch_bwd(const BwdArgs &a, cudaStream_t s) {
-  // shares of a row: eight blocks' worth on each SM of a B200 while a thread has two granules
+int launch_fwd(const FwdArgs &a, cudaStream_t s) {
+  // A row's fixed work (its joins) is per warp: few threads for short rows (8192 rows of 4000
+  // bf16 values: 29 us with 32 threads, 34 with 128; of 10000: 66 with 128, 84 with 256).
+  const int granules = (a.V + kPer<T> - 1) / kPer<T>;
+  if (granules <= 512) return launch_fwd_threads<T, 32>(a, s);
+  if (granules <= 2048) return launch_fwd_threads<T, 128>(a, s);
+  return launch_fwd_threads<T, 256>(a, s);
+}
+
+template <typename T, int kNT>
+int launch_bwd_threads(const BwdArgs &a, cudaStream_t s) {
+  // shares of a row: sixteen blocks' worth on each SM of a B200 while a thread has two granules
   long long C = 1;
-  while (a.rows * C < 8 * 148 && a.V >= 4 * C * kNT * kPer<T>) C *= 2;
+  while (a.rows * C < 16 * 148 && a.V >= 4 * C * kNT * kPer<T>) C *= 2;
   const dim3 grid((unsigned)a.rows, (unsigned)C);
   const uintptr_t l = reinterpret_cast<uintptr_t>(a.logits), d = reinterpret_cast<uintptr_t>(a.dlogits);
   if (((l ^ d) & 15) == 0 && (a.stride - a.V) % kPer<T> == 0) {
     if (a.g_entropy)
-      logprobs_bwd_kernel<T, true><<<grid, kNT, 0, s>>>(a);
+      logprobs_bwd_kernel<T, true, kNT><<<grid, kNT, 0, s>>>(a);
     else
-      logprobs_bwd_kernel<T, false><<<grid, kNT, 0, s>>>(a);
+      logprobs_bwd_kernel<T, false, kNT><<<grid, kNT, 0, s>>>(a);
   } else {
-    logprobs_bwd_loop_kernel<T><<<grid, kNT, 0, s>>>(a);
+    logprobs_bwd_loop_kernel<T, kNT><<<grid, kNT, 0, s>>>(a);
   }
   return launched("token_logprobs_bwd");
+}
+
+template <typename T>
+int launch_bwd(const BwdArgs &a, cudaStream_t s) {
+  return (a.V + kPer<T> - 1) / kPer<T> <= 512 ? launch_bwd_threads<T, 64>(a, s) : launch_bwd_threads<T, 256>(a, s);
 }
 
 int check_shape(int64_t rows, int64_t V, int64_t stride, int dtype, float temperature) {
