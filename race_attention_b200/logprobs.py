@@ -23,19 +23,26 @@ class TokenLogprobsFn(torch.autograd.Function):
     def forward(ctx, logits, tokens, temperature, n_top, ignore_index):
         logp, entropy, lse, top_ids, top_logp = ops.token_logprobs_fwd(logits, tokens, temperature, n_top, ignore_index)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, tokens, lse, entropy)
+        ctx.save_for_backward(logits, tokens.contiguous(), lse, entropy)
         ctx.temperature, ctx.ignore_index = temperature, ignore_index
         ctx.mark_non_differentiable(top_ids, top_logp)
         return logp, entropy, top_ids, top_logp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy, _ids, _top):
-        logits, tokens, lse, entropy = ctx.saved_tensors
-        if g_logp is None and g_entropy is None:
-            return None, None, None, None, None
-        return ops.token_logprobs_bwd(logits, tokens, lse, entropy, g_logp, g_entropy, ctx.temperature,
-                                      ctx.ignore_index), None, None, None, None
+        # (the guard against a second differentiation only where a graph of this one is made)
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, g_logp, g_entropy)
+
+
+def _backward(ctx, g_logp, g_entropy):
+    logits, tokens, lse, entropy = ctx.saved_tensors
+    if g_logp is None and g_entropy is None:
+        return None, None, None, None, None
+    return ops.token_logprobs_bwd_unchecked(logits, tokens, lse, entropy, g_logp, g_entropy, ctx.temperature,
+                                            ctx.ignore_index), None, None, None, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def token_logprobs(logits, tokens, temperature=1.0, n_top=0, ignore_index=-100) -> TokenLogprobs:

@@ -17,20 +17,27 @@ class AddRMSNormFn(torch.autograd.Function):
     def forward(ctx, x, residual, weight, eps):
         y, h, rstd = ops.rms_norm_fwd(x, residual, weight, eps, return_rstd=True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(h, rstd, weight)
         ctx.has_residual = residual is not None
+        ctx.save_for_backward(h, rstd, weight)
         return (y, h) if ctx.has_residual else y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh=None):
-        h, rstd, weight = ctx.saved_tensors
-        dw = None
-        if dy is None:  # only h was used
-            dx = dh
-        else:
-            dx, dw = ops.rms_norm_bwd(dy, dh, h, rstd, weight, ctx.needs_input_grad[2])
-        return dx, dx if ctx.has_residual else None, dw, None
+        # (the guard against a second differentiation only where a graph of this one is made)
+        return _backward_once(ctx, dy, dh) if torch.is_grad_enabled() else _backward(ctx, dy, dh)
+
+
+def _backward(ctx, dy, dh):
+    h, rstd, weight = ctx.saved_tensors
+    dw = None
+    if dy is None:  # only h was used
+        dx = dh
+    else:
+        dx, dw = ops.rms_norm_bwd_unchecked(dy, dh, h.contiguous(), rstd, weight, ctx.needs_input_grad[2])
+    return dx, dx if ctx.has_residual else None, dw, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def add_rms_norm(x, residual=None, weight=None, eps=1e-5):

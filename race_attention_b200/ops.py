@@ -512,16 +512,18 @@ def gqa_decode_attention(q, k_new, v_new, k_cache, v_cache, length, workspace, n
 
 # ---------------------------------------------------------------------------
 # operators around the layer: residual RMS norm, 8-bit rows and products, token log
-# probabilities.  Some of them run for a few microseconds on a decode step, so they
-# launch without entering a device context where the tensors' device is current.
+# probabilities.  Some of them run for a few microseconds on a decode step, so their checks
+# are single passes over attributes and they launch without entering a device context where
+# the tensors' device is current.
 def _launch(dev, name, *args):
     """Call C entry point `name` with args and the current stream of `dev`."""
     fn = getattr(_lib.load(), name)
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, name)
 
@@ -553,10 +555,12 @@ def _weight_code(weight, K):
 def _norm_inputs(x, residual, weight):
     dev = _check_cuda(x, residual, weight)
     code = _dtype_code(x)
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise RuntimeError("residual must have x's shape and dtype")
     xr, xs, rows, K = _rows(x, "x")
-    rr, rs = (None, 0) if residual is None else _rows(residual, "residual")[:2]
+    rr, rs = None, 0
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise RuntimeError("residual must have x's shape and dtype")
+        rr, rs, _, _ = _rows(residual, "residual")
     return dev, code, xr, xs, rr, rs, rows, K, _weight_code(weight, K)
 
 
@@ -564,13 +568,17 @@ def _ptr_of(t):
     return None if t is None else t.data_ptr()
 
 
+def _dense_like(x):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def rms_norm_fwd(x, residual=None, weight=None, eps=1e-5, return_rstd=False):
     """(y, h[, rstd]): h = x + residual in x's dtype (x itself without a residual),
     y = h * rsqrt(mean(h^2) + eps) * weight; x [..., K]."""
     dev, code, xr, xs, rr, rs, rows, K, wc = _norm_inputs(x, residual, weight)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if return_rstd else None
+    y = _dense_like(x)
+    h = x if residual is None else _dense_like(x)
+    rstd = x.new_empty(rows, dtype=torch.float32) if return_rstd else None
     if rows:
         _launch(dev, "race_rms_norm_fwd", xr.data_ptr(), xs, _ptr_of(rr), rs, code, _ptr_of(weight), wc, y.data_ptr(),
                 None if residual is None else h.data_ptr(), _ptr_of(rstd), rows, K, eps)
@@ -580,51 +588,54 @@ def rms_norm_fwd(x, residual=None, weight=None, eps=1e-5, return_rstd=False):
 def rms_norm_bwd(dy, dh, h, rstd, weight=None, weight_grad=True):
     """(dx, dw) of rms_norm_fwd for the gradients dy of y and dh of h (None: zero); dx is the
     gradient of x and of the residual alike, dw (None unless weight_grad) has weight's dtype."""
-    dev = _check_cuda(dy, dh, h, rstd, weight)
-    code = _dtype_code(h)
-    K = h.shape[-1]
+    _check_cuda(dy, dh, h, rstd, weight)
     if dy.shape != h.shape or dy.dtype != h.dtype or (dh is not None and (dh.shape != h.shape or dh.dtype != h.dtype)):
         raise RuntimeError("dy and dh must have h's shape and dtype")
+    if rstd.dtype != torch.float32 or rstd.numel() * h.shape[-1] != h.numel():
+        raise RuntimeError(f"rstd must hold {h.numel() // h.shape[-1]} float32 values")
+    _weight_code(weight, h.shape[-1])
+    return rms_norm_bwd_unchecked(dy, dh, h.contiguous(), rstd.contiguous(), weight, weight_grad)
+
+
+def rms_norm_bwd_unchecked(dy, dh, h, rstd, weight, weight_grad):
+    """rms_norm_bwd for what autograd saved and checked (h and rstd dense)."""
+    K = h.shape[-1]
     rows = h.numel() // K
-    if rstd.dtype != torch.float32 or rstd.numel() != rows:
-        raise RuntimeError(f"rstd must hold {rows} float32 values")
-    wc = _weight_code(weight, K)
-    dy, h, rstd = dy.contiguous(), h.contiguous(), rstd.contiguous()
-    dh = None if dh is None else dh.contiguous()
-    dx = torch.empty(h.shape, dtype=h.dtype, device=dev)
+    dy = dy.contiguous()
+    dx = torch.empty_like(h)
     dw = ws = None
     nb = 0
     if weight_grad:
-        dw = torch.empty(K, dtype=torch.float32 if weight is None else weight.dtype, device=dev)
-        nb = int(_lib.load().race_rms_norm_bwd_workspace_bytes(rows, K)) if rows else 0
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+        dw = h.new_empty(K, dtype=torch.float32) if weight is None else torch.empty_like(weight)
+        if not rows:
+            dw.zero_()
+        else:
+            nb = _lib.load().race_rms_norm_bwd_workspace_bytes(rows, K)
+            ws = h.new_empty(nb, dtype=torch.uint8)
     if rows:
-        _launch(dev, "race_rms_norm_bwd", dy.data_ptr(), _ptr_of(dh), h.data_ptr(), rstd.data_ptr(), code,
-                _ptr_of(weight), wc, dx.data_ptr(), _ptr_of(dw), rows, K, _ptr_of(ws), nb)
-    elif dw is not None:
-        dw.zero_()
+        dh = None if dh is None else dh.contiguous()
+        _launch(h.device, "race_rms_norm_bwd", dy.data_ptr(), _ptr_of(dh), h.data_ptr(), rstd.data_ptr(), _dtype_code(h),
+                _ptr_of(weight), _lib.RACE_F32 if weight is None else _dtype_code(weight), dx.data_ptr(), _ptr_of(dw),
+                rows, K, _ptr_of(ws), nb)
     return dx, dw
 
 
-def _int8_out(shape, dev):
-    """8-bit rows [..., K] whose rows start at multiples of 16 bytes (what the 8-bit product's
-    tile loads need), their row stride, and their scales [...]."""
-    K = shape[-1]
-    rows = math.prod(shape[:-1])
+def _int8_out(x, K):
+    """8-bit rows [..., K] (for x [..., *]) that start at multiples of 16 bytes, as the 8-bit
+    product's tile loads need, their row stride, and their scales [...]."""
+    lead = x.shape[:-1]
+    scale = x.new_empty(lead, dtype=torch.float32)
+    if K % 16 == 0:
+        return x.new_empty(lead + (K,), dtype=torch.int8), K, scale
     stride = -(-K // 16) * 16
-    q = torch.empty((rows, stride), dtype=torch.int8, device=dev)
-    if stride != K:
-        q = q[:, :K]
-    if len(shape) != 2:
-        q = q.unflatten(0, shape[:-1]) if len(shape) > 2 else q[0]
-    return q, stride, torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    return x.new_empty(lead + (stride,), dtype=torch.int8)[..., :K], stride, scale
 
 
 def rms_norm_int8(x, residual=None, weight=None, eps=1e-5):
     """(q, scale, h): the y of rms_norm_fwd as 8-bit rows (not rounded in between), and h."""
     dev, code, xr, xs, rr, rs, rows, K, wc = _norm_inputs(x, residual, weight)
-    q, qs, scale = _int8_out(x.shape, dev)
-    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    q, qs, scale = _int8_out(x, K)
+    h = x if residual is None else _dense_like(x)
     if rows:
         _launch(dev, "race_rms_norm_int8", xr.data_ptr(), xs, _ptr_of(rr), rs, code, _ptr_of(weight), wc, q.data_ptr(),
                 qs, scale.data_ptr(), None if residual is None else h.data_ptr(), rows, K, eps)
@@ -636,7 +647,7 @@ def quant_int8(x):
     dev = _check_cuda(x)
     code = _dtype_code(x)
     xr, xs, rows, K = _rows(x, "x")
-    q, qs, scale = _int8_out(x.shape, dev)
+    q, qs, scale = _int8_out(x, K)
     if rows:
         _launch(dev, "race_quant_int8", xr.data_ptr(), xs, code, q.data_ptr(), qs, scale.data_ptr(), rows, K)
     return q, scale
@@ -649,7 +660,7 @@ def swiglu_int8(gate_up):
     xr, xs, rows, K2 = _rows(gate_up, "gate_up")
     if K2 % 2:
         raise RuntimeError("gate_up must hold an even number of values per row")
-    q, qs, scale = _int8_out(gate_up.shape[:-1] + (K2 // 2,), dev)
+    q, qs, scale = _int8_out(gate_up, K2 // 2)
     if rows:
         _launch(dev, "race_swiglu_int8", xr.data_ptr(), xs, code, q.data_ptr(), qs, scale.data_ptr(), rows, K2 // 2)
     return q, scale
@@ -665,7 +676,7 @@ def dequant_int8(q, scale, dtype=torch.bfloat16):
     """q * scale, rounded to dtype."""
     dev = _check_cuda(q, scale)
     qr, qs, rows, K, scale = _int8_rows(q, scale, "q")
-    out = torch.empty(q.shape, dtype=dtype, device=dev)
+    out = q.new_empty(q.shape, dtype=dtype)
     if rows:
         _launch(dev, "race_dequant_int8", qr.data_ptr(), qs, scale.data_ptr(), out.data_ptr(), _dtype_code(out), rows, K)
     return out
@@ -677,7 +688,7 @@ def _aligned_rows(q, stride):
         return q, stride
     K = q.shape[-1]
     stride = -(-K // 16) * 16
-    p = torch.empty((q.numel() // K, stride), dtype=torch.int8, device=q.device)[:, :K]
+    p = q.new_empty((q.numel() // K, stride))[:, :K]
     p.copy_(q.reshape(-1, K))
     return p, stride
 
@@ -693,8 +704,8 @@ def int8_linear(xq, x_scale, wq, w_scale, bias=None, dtype=torch.bfloat16):
     wr, ws, N, _, w_scale = _int8_rows(wq, w_scale, "w")
     if bias is not None and (bias.shape != (N,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
         raise RuntimeError(f"bias must be a contiguous float32 [{N}] tensor")
-    y = torch.empty(xq.shape[:-1] + (N,), dtype=dtype, device=dev)
-    code = _dtype_code(y)
+    code = _dtype_code_of(dtype)
+    y = xq.new_empty(xq.shape[:-1] + (N,), dtype=dtype)
     if M and N:
         xr, xs = _aligned_rows(xr, xs)
         wr, ws = _aligned_rows(wr, ws)
@@ -716,11 +727,11 @@ def token_logprobs_fwd(logits, tokens, temperature=1.0, n_top=0, ignore_index=-1
     dev, code, lr, ls, rows, V, tokens = _logit_rows(logits, tokens)
     n_top = int(n_top)
     shape = tokens.shape
-    logp = torch.empty(shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty(shape, dtype=torch.float32, device=dev)
-    lse = torch.empty(shape + (2,), dtype=torch.float32, device=dev)
-    top_ids = torch.empty(shape + (max(n_top, 0),), dtype=torch.int64, device=dev)
-    top_logp = torch.empty(shape + (max(n_top, 0),), dtype=torch.float32, device=dev)
+    logp = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(logp)
+    lse = logp.new_empty(shape + (2,))
+    top_logp = logp.new_empty(shape + (max(n_top, 0),))
+    top_ids = torch.empty_like(top_logp, dtype=torch.int64)
     if rows:
         _launch(dev, "race_token_logprobs_fwd", lr.data_ptr(), ls, code, tokens.data_ptr(), int(ignore_index),
                 float(temperature), n_top, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top_ids.data_ptr(),
@@ -730,15 +741,24 @@ def token_logprobs_fwd(logits, tokens, temperature=1.0, n_top=0, ignore_index=-1
 
 def token_logprobs_bwd(logits, tokens, lse, entropy, g_logp, g_entropy, temperature=1.0, ignore_index=-100):
     """dlogits of token_logprobs_fwd for the gradients g_logp, g_entropy (None: zero)."""
-    dev, code, lr, ls, rows, V, tokens = _logit_rows(logits, tokens)
+    _logit_rows(logits, tokens)
     _check_cuda(logits, lse, entropy, g_logp, g_entropy)
-    lse, entropy, g_logp, g_entropy = (None if t is None else t.float().contiguous()
-                                       for t in (lse, entropy, g_logp, g_entropy))
-    if lse.numel() != 2 * rows or any(t is not None and t.numel() != rows for t in (entropy, g_logp, g_entropy)):
+    rows = tokens.numel()
+    if lse.numel() != 2 * rows or entropy.numel() != rows or (g_logp is not None and g_logp.numel() != rows) \
+            or (g_entropy is not None and g_entropy.numel() != rows):
         raise RuntimeError(f"lse must hold {2 * rows} values, entropy and the gradients {rows}")
-    d = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    return token_logprobs_bwd_unchecked(logits, tokens.contiguous(), lse.float().contiguous(), entropy.float().contiguous(),
+                                        g_logp, g_entropy, temperature, ignore_index)
+
+
+def token_logprobs_bwd_unchecked(logits, tokens, lse, entropy, g_logp, g_entropy, temperature, ignore_index):
+    """token_logprobs_bwd for what autograd saved and checked (dense but for the logits)."""
+    lr, ls, rows, V = _rows(logits, "logits")
+    g_logp = None if g_logp is None else g_logp.float().contiguous()
+    g_entropy = None if g_entropy is None else g_entropy.float().contiguous()
+    d = _dense_like(logits)
     if rows:
-        _launch(dev, "race_token_logprobs_bwd", lr.data_ptr(), ls, code, tokens.data_ptr(), int(ignore_index),
-                float(temperature), lse.data_ptr(), entropy.data_ptr(), _ptr_of(g_logp), _ptr_of(g_entropy),
-                d.data_ptr(), rows, V)
+        _launch(logits.device, "race_token_logprobs_bwd", lr.data_ptr(), ls, _dtype_code(logits), tokens.data_ptr(),
+                int(ignore_index), float(temperature), lse.data_ptr(), entropy.data_ptr(), _ptr_of(g_logp),
+                _ptr_of(g_entropy), d.data_ptr(), rows, V)
     return d
