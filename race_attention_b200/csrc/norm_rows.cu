@@ -654,13 +654,45 @@ __global__ void __launch_bounds__(1024) dw_sum_kernel(const float *part, int n, 
   }
 }
 
+// Rows of 8 bits back to values: a thread writes the 8 values of an output vector (a granule of
+// bf16, two of fp32; skewed as the rows of `out` lie, see kSkewed), from the one or two aligned
+// 8-byte words of q that hold their bytes.  blockDim.y rows per block.
 template <typename T>
-__global__ void __launch_bounds__(256) dequant_kernel(const int8_t *q, long long q_stride, const float *scale, T *out,
-                                                      long long rows, int K) {
-  const long long row = blockIdx.x;
-  const float s = scale[row];
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < K; i += gridDim.y * 256)
-    out[row * K + i] = from_f<T>((float)q[row * q_stride + i] * s);
+__global__ void __launch_bounds__(256) dequant_kernel(const int8_t *q_rows, long long q_stride, const float *scale, T *out,
+                                                      long long rows, int K, bool q_vec) {
+  const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= rows) return;
+  const float s = __ldg(scale + row);
+  const int8_t *q = q_rows + row * q_stride;
+  T *o = out + row * K;
+  const int off = misalign(o);
+  for (int e = threadIdx.x * 8 - off; e < K; e += blockDim.x * 8) {
+    const int w = e & ~7, shift = 8 * (e & 3);  // the word that holds byte e
+    uint32_t lo = 0, hi = 0;
+    if (q_vec && w >= 0 && w + (off ? 16 : 8) <= K) {
+      const uint2 a = __ldg(reinterpret_cast<const uint2 *>(q + w));
+      uint2 b = make_uint2(0, 0);
+      if (off) b = __ldg(reinterpret_cast<const uint2 *>(q + w + 8));
+      const bool half = e & 4;
+      const uint32_t c0 = half ? a.y : a.x, c1 = half ? b.x : a.y, c2 = half ? b.y : b.x;
+      lo = __funnelshift_r(c0, c1, shift);
+      hi = __funnelshift_r(c1, c2, shift);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (e + k >= 0 && e + k < K) {
+          const uint32_t v = (uint32_t)(uint8_t)__ldg(q + e + k) << (8 * (k & 3));
+          if (k < 4)
+            lo |= v;
+          else
+            hi |= v;
+        }
+    }
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = (float)(int8_t)((k < 4 ? lo : hi) >> (8 * (k & 3))) * s;
+    store8<T, kSkewed>(o, e, K, f);
+  }
 }
 
 // ------------------------------------------------------------------ host side
@@ -863,14 +895,19 @@ int race_swiglu_int8(const void *gate_up, int64_t stride, int dtype, int8_t *q, 
 int race_dequant_int8(const int8_t *q, int64_t q_stride, const float *scale, void *out, int dtype, int64_t rows,
                       int64_t K, void *stream) {
   if (!q || !scale || !out) return err(RACE_ERR_ARG, "race_dequant_int8: null pointer");
-  if (const int rc = check_rows("race_dequant_int8", rows, K, dtype)) return rc;
+  if (const int rc = check_rows("race_dequant_int8", rows, K, dtype, {out})) return rc;
   if (q_stride < K) return err(RACE_ERR_SHAPE, "race_dequant_int8: row stride below the width %lld", K);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)rows, (unsigned)((K + 1023) / 1024 < 64 ? (K + 1023) / 1024 : 64));
+  // rows of up to 2048 values share a block of 256 threads
+  int x = 1;
+  while (x < 256 && x * 8 < K + 7) x *= 2;
+  const dim3 block((unsigned)x, (unsigned)(256 / x));
+  const unsigned grid = (unsigned)((rows + block.y - 1) / block.y);
+  const bool q_vec = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)q_stride) & 7) == 0;
   if (dtype == RACE_BF16)
-    dequant_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(q, q_stride, scale, static_cast<__nv_bfloat16 *>(out), rows, (int)K);
+    dequant_kernel<<<grid, block, 0, s>>>(q, q_stride, scale, static_cast<__nv_bfloat16 *>(out), rows, (int)K, q_vec);
   else
-    dequant_kernel<float><<<grid, 256, 0, s>>>(q, q_stride, scale, static_cast<float *>(out), rows, (int)K);
+    dequant_kernel<<<grid, block, 0, s>>>(q, q_stride, scale, static_cast<float *>(out), rows, (int)K, q_vec);
   return launched("dequant_int8");
 }
 

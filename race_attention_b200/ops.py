@@ -684,9 +684,12 @@ def dequant_int8(q, scale, dtype=torch.bfloat16):
 
 def _aligned_rows(q, stride):
     """8-bit rows whose starts are multiples of 16 bytes: q, or a padded copy of it."""
-    if stride % 16 == 0 and q.data_ptr() % 16 == 0:
-        return q, stride
     K = q.shape[-1]
+    if q.data_ptr() % 16 == 0:
+        if stride % 16 == 0:
+            return q, stride
+        if q.numel() == K:  # a single row: nothing lies a stride further on
+            return q, -(-K // 16) * 16
     stride = -(-K // 16) * 16
     p = q.new_empty((q.numel() // K, stride))[:, :K]
     p.copy_(q.reshape(-1, K))
