@@ -421,7 +421,8 @@ int race_dequant_int8(const int8_t *q, int64_t q_stride, const float *scale, voi
  * xq, wq and their row strides (bytes) must be multiples of 16 (else RACE_ERR_ALIGN):
  * the tiles come in by TMA.  Its device-side waits are bounded like the layer's
  * (race_set_wait_limit); there is no workspace, so a call whose wait gave up writes NaN,
- * and under race_set_status_check(1) returns RACE_ERR_TIMEOUT. */
+ * and under race_set_status_check(1) returns RACE_ERR_TIMEOUT (unless the stream is being
+ * captured, where nothing runs that could be waited for). */
 int race_int8_linear(const int8_t *xq, int64_t x_stride, const float *x_scale, const int8_t *wq, int64_t w_stride,
                      const float *w_scale, const float *bias, void *y, int dtype, int64_t M, int64_t N, int64_t K,
                      void *stream);

@@ -642,11 +642,16 @@ int launch(const int8_t *xq, int64_t x_stride, const int8_t *wq, int64_t w_strid
   }
 }
 
-// race_set_status_check(1): wait for the stream and report a wait that gave up.
+// race_set_status_check(1): wait for the stream and report a wait that gave up (a captured call
+// does not run now, so there is nothing to wait for).
 int check_status(cudaStream_t s) {
   if (!race::status_check_on()) return RACE_OK;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(s, &capture);
+  if (e != cudaSuccess) return cuda_err("int8_linear", e);
+  if (capture != cudaStreamCaptureStatusNone) return RACE_OK;
   int flag = 0;
-  cudaError_t e = cudaStreamSynchronize(s);
+  e = cudaStreamSynchronize(s);
   if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&flag, g_timeout, sizeof(flag));
   if (e != cudaSuccess) return cuda_err("int8_linear", e);
   if (!flag) return RACE_OK;

@@ -8,7 +8,10 @@ embedding and QK norm in the attention, planes of layer i seeded with i
 takes q, k, v in the [B, T, H, D] layout the projections produce (nanochat_race_attention:
 no transposes).  Value embeddings, sliding windows and the KV cache of the reference model
 are not part of this harness.  Linear layers keep fp32 master weights and run in the
-activation dtype (bf16).
+activation dtype (bf16).  With GPTConfig.fused the blocks' residual additions and norms are one
+kernel each (add_rms_norm), and the loss comes from token_logprobs, which reads the logits in
+their own type and keeps no fp32 copy of them; token_logprobs() gives the same for losses on
+log probabilities and entropies (policy gradients, distillation).
 """
 from __future__ import annotations
 
@@ -18,6 +21,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .logprobs import token_logprobs
+from .norm import add_rms_norm
 from .race_causal_cuda import nanochat_race_attention
 from .race_common import build_planes_protos
 
@@ -33,6 +38,8 @@ class GPTConfig:
     race_P: int = 4
     race_eps: float = 1e-6
     rope_base: float = 10000.0
+    fused: bool = False        # add_rms_norm in the blocks, token_logprobs for the loss
+    norm_eps: float = 1e-6     # of the fused norms
 
 
 def _rms(x):
@@ -96,6 +103,13 @@ class Block(nn.Module):
         x = x + self.attn(_rms(x), cos, sin)
         return x + self.mlp(_rms(x))
 
+    def forward_fused(self, d, x, cos, sin, eps):
+        """The residual stream x and what is still to be added to it (d, None in front of the first
+        block), to both after the block."""
+        y, x = add_rms_norm(x, None, None, eps) if d is None else add_rms_norm(d, x, None, eps)
+        y, x = add_rms_norm(self.attn(y, cos, sin), x, None, eps)
+        return self.mlp(y), x
+
 
 class RaceGPT(nn.Module):
     def __init__(self, cfg: GPTConfig):
@@ -115,13 +129,27 @@ class RaceGPT(nn.Module):
         ang = torch.outer(torch.arange(T, device=device, dtype=torch.float32), inv)
         return ang.cos().to(dtype)[None, :, None, :], ang.sin().to(dtype)[None, :, None, :]
 
-    def forward(self, idx, targets=None, dtype=torch.bfloat16):
+    def logits(self, idx, dtype=torch.bfloat16):
         B, T = idx.shape
         cos, sin = self._angles(T, idx.device, dtype)
         x = _rms(self.wte(idx).to(dtype))
+        if self.cfg.fused:
+            d = None
+            for blk in self.blocks:
+                d, x = blk.forward_fused(d, x, cos, sin, self.cfg.norm_eps)
+            return self.lm_head(add_rms_norm(d, x, None, self.cfg.norm_eps)[0])
         for blk in self.blocks:
             x = blk(x, cos, sin)
-        logits = self.lm_head(_rms(x))
+        return self.lm_head(_rms(x))
+
+    def token_logprobs(self, idx, targets, temperature=1.0, n_top=0, dtype=torch.bfloat16):
+        """TokenLogprobs of targets [B, T] (-100: none) after idx [B, T], differentiable."""
+        return token_logprobs(self.logits(idx, dtype), targets, temperature, n_top)
+
+    def forward(self, idx, targets=None, dtype=torch.bfloat16):
+        logits = self.logits(idx, dtype)
         if targets is None:
             return logits
+        if self.cfg.fused:
+            return -token_logprobs(logits, targets).logp.sum() / (targets != -100).sum()
         return F.cross_entropy(logits.float().view(-1, logits.size(-1)), targets.view(-1))

@@ -12,6 +12,12 @@ decode step depends on host-side position values, DecodeGraph captures one whole
 CUDA graph and replays it.  Architecture: 16 layers, hidden 2048, 32 / 8 heads, head_dim 64,
 SwiGLU MLP 8192, RMSNorm (eps 1e-5), RoPE theta 500000, vocabulary 128256 with the LM head
 tied to the embedding.  Decoding runs in bf16 (the softmax layers' kernel is bf16-only).
+
+quantize_int8() turns the projections, the MLP and the LM head into 8-bit layers.  Every residual
+addition, norm and quantisation in front of a projection is then one kernel (add_rms_norm_int8:
+a block hands the next one its unadded output), and the MLP's activation one (swiglu_int8).
+score() and step_logprobs() give the log probabilities of given and of decoded tokens with their
+entropies and alternatives (token_logprobs), in either form.
 """
 from __future__ import annotations
 
@@ -23,6 +29,8 @@ import torch.nn.functional as F
 
 from . import ops
 from .decode import RaceDecodeState, prefill_with_state
+from .int8 import Int8Linear, add_rms_norm_int8, swiglu_int8
+from .logprobs import token_logprobs
 from .race_common import build_planes_protos
 
 
@@ -79,8 +87,15 @@ class Layer(nn.Module):
         self.cache = None      # softmax layers: (K, V) [B, Hkv, Tmax, D]
         self.attn_ws = None    # softmax layers: race_gqa_decode_attn workspace and its split count
         self.n_splits = 1
+        self.int8 = False
+
+    def quantize_int8(self):
+        self.qkv, self.o, self.gate_up, self.down = (Int8Linear.from_linear(m) for m in
+                                                     (self.qkv, self.o, self.gate_up, self.down))
+        self.int8 = True
 
     def _qkv(self, x, cos, sin):
+        """x [B, T, hidden], or its 8-bit rows."""
         B, T, _ = x.shape
         cfg, hd = self.cfg, self.hd
         q, k, v = self.qkv(x).view(B, T, cfg.n_head + 2 * cfg.n_kv_head, hd).split(
@@ -96,14 +111,19 @@ class Layer(nn.Module):
         """x [mb, T, hidden]: sequences [b0, b0 + mb) of a batch of `batch`, from position 0;
         fills their slice of the layer's decode state / KV cache (allocated on b0 == 0)."""
         mb, T, _ = x.shape
+        y = self._attend_prefill(*self._qkv(self.ln1(x), cos, sin), t_max, b0, batch)
+        x = x + self.o(y.transpose(1, 2).reshape(mb, T, -1))
+        return x + self._mlp(self.ln2(x))
+
+    def _attend_prefill(self, q, k, v, t_max, b0, batch):
+        mb, T = q.shape[0], q.shape[2]
         cfg = self.cfg
-        q, k, v = self._qkv(self.ln1(x), cos, sin)
         if self.race:
             y, st = prefill_with_state(q.contiguous(), k.contiguous(), v.contiguous(), self.planes_T, cfg.race_L,
                                        cfg.race_P, cfg.race_eps)
             if b0 == 0:
                 self.state = RaceDecodeState(batch, cfg.n_kv_head, self.hd, cfg.race_L, cfg.race_P, self.planes_T,
-                                             cfg.race_eps, device=x.device)
+                                             cfg.race_eps, device=q.device)
             rows = slice(b0 * cfg.n_kv_head, (b0 + mb) * cfg.n_kv_head)
             self.state.A[rows].copy_(st.A)
             self.state.B[rows].copy_(st.B)
@@ -117,20 +137,39 @@ class Layer(nn.Module):
             self.cache[0][b0:b0 + mb, :, :T].copy_(k)
             self.cache[1][b0:b0 + mb, :, :T].copy_(v)
             y = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
-        x = x + self.o(y.transpose(1, 2).reshape(mb, T, -1))
-        return x + self._mlp(self.ln2(x))
+        return y
 
     def step(self, x, cos, sin, pos):
         """x [B, 1, hidden] at position pos (int32 device tensor [1] = tokens already seen)."""
         B = x.shape[0]
-        q, k, v = self._qkv(self.ln1(x), cos, sin)  # [B, H, 1, D]
-        q, k, v = q[:, :, 0].contiguous(), k[:, :, 0].contiguous(), v[:, :, 0].contiguous()
-        if self.race:
-            y = self.state.step(q, k, v)
-        else:
-            y = ops.gqa_decode_attention(q, k, v, self.cache[0], self.cache[1], pos, self.attn_ws, self.n_splits)
+        y = self._attend_step(*self._qkv(self.ln1(x), cos, sin), pos)
         x = x + self.o(y.reshape(B, 1, -1))
         return x + self._mlp(self.ln2(x))
+
+    def _attend_step(self, q, k, v, pos):  # [B, H, 1, D]
+        q, k, v = q[:, :, 0].contiguous(), k[:, :, 0].contiguous(), v[:, :, 0].contiguous()
+        if self.race:
+            return self.state.step(q, k, v)
+        return ops.gqa_decode_attention(q, k, v, self.cache[0], self.cache[1], pos, self.attn_ws, self.n_splits)
+
+    # The 8-bit forms take the residual stream x and what is still to be added to it (d, None in
+    # front of the first layer), and return both again.
+    def _rows(self, ln, d, x):
+        return add_rms_norm_int8(x, None, ln.weight, ln.eps) if d is None else add_rms_norm_int8(d, x, ln.weight, ln.eps)
+
+    def _mlp_int8(self, d, x):
+        rows, x = self._rows(self.ln2, d, x)
+        return self.down(swiglu_int8(self.gate_up(rows))), x
+
+    def prefill_int8(self, d, x, cos, sin, t_max, b0, batch):
+        rows, x = self._rows(self.ln1, d, x)
+        y = self._attend_prefill(*self._qkv(rows, cos, sin), t_max, b0, batch)
+        return self._mlp_int8(self.o(y.transpose(1, 2).reshape(x.shape[0], x.shape[1], -1)), x)
+
+    def step_int8(self, d, x, cos, sin, pos):
+        rows, x = self._rows(self.ln1, d, x)
+        y = self._attend_step(*self._qkv(rows, cos, sin), pos)
+        return self._mlp_int8(self.o(y.reshape(x.shape[0], 1, -1)), x)
 
 
 class HybridLlama(nn.Module):
@@ -143,6 +182,7 @@ class HybridLlama(nn.Module):
         self.pos = None        # int32 device tensor [1]: tokens in the decode state / caches
         self.n_tokens = 0      # the same count on the host
         self.t_max = 0
+        self.head = None       # 8-bit LM head (quantize_int8); else tied to the embedding
 
     def init_weights(self, std=0.02):
         for name, p in self.named_parameters():
@@ -157,8 +197,37 @@ class HybridLlama(nn.Module):
         ang = torch.outer(torch.arange(pos0, pos0 + T, device=device, dtype=torch.float32), self._inv_freq(device))
         return ang.cos().to(dtype), ang.sin().to(dtype)
 
+    @torch.no_grad()
+    def quantize_int8(self):
+        """Projections, MLP and LM head as 8-bit layers, in place (the embedding stays as it is)."""
+        for layer in self.layers:
+            layer.quantize_int8()
+        self.head = Int8Linear(self.embed.weight, dtype=self.embed.weight.dtype)
+        return self
+
     def _logits(self, x):
         return F.linear(self.norm(x), self.embed.weight)
+
+    def _prefill_hidden(self, x, cos, sin, t_max, b0, batch):
+        """The layers over embedded tokens x; a function from a slice of positions to their logits."""
+        if self.head is None:
+            for layer in self.layers:
+                x = layer.prefill(x, cos, sin, t_max, b0, batch)
+            return lambda at: self._logits(x[:, at])
+        d = None
+        for layer in self.layers:
+            d, x = layer.prefill_int8(d, x, cos, sin, t_max, b0, batch)
+        return lambda at: self.head(add_rms_norm_int8(d[:, at], x[:, at], self.norm.weight, self.norm.eps)[0])
+
+    def _forward_only(self, idx):
+        """_prefill_hidden over idx [B, T] that leaves the decode state and caches as they were."""
+        B, T = idx.shape
+        kept = [(layer.state, layer.cache, layer.attn_ws, layer.n_splits) for layer in self.layers]
+        cos, sin = self._angles(0, T, idx.device, self.embed.weight.dtype)
+        logits = self._prefill_hidden(self.embed(idx), cos, sin, T, 0, B)
+        for layer, (st, cache, ws, ns) in zip(self.layers, kept):
+            layer.state, layer.cache, layer.attn_ws, layer.n_splits = st, cache, ws, ns
+        return logits
 
     @torch.no_grad()
     def prefill(self, idx, t_max, micro_batch=4):
@@ -168,10 +237,8 @@ class HybridLlama(nn.Module):
         cos, sin = self._angles(0, T, idx.device, self.embed.weight.dtype)
         nxt = []
         for b0 in range(0, B, micro_batch):
-            x = self.embed(idx[b0:b0 + micro_batch])
-            for layer in self.layers:
-                x = layer.prefill(x, cos, sin, t_max, b0, B)
-            nxt.append(self._logits(x[:, -1]).argmax(-1))
+            logits = self._prefill_hidden(self.embed(idx[b0:b0 + micro_batch]), cos, sin, t_max, b0, B)
+            nxt.append(logits(-1).argmax(-1))
         self.pos = torch.full((1,), T, dtype=torch.int32, device=idx.device)
         self.n_tokens, self.t_max = T, t_max
         return torch.cat(nxt)
@@ -179,15 +246,17 @@ class HybridLlama(nn.Module):
     @torch.no_grad()
     def logits_full(self, idx):
         """Last-position logits of a plain causal forward over idx [B, T] (no caches kept)."""
-        B, T = idx.shape
-        kept = [(layer.state, layer.cache, layer.attn_ws, layer.n_splits) for layer in self.layers]
-        cos, sin = self._angles(0, T, idx.device, self.embed.weight.dtype)
-        x = self.embed(idx)
-        for layer in self.layers:
-            x = layer.prefill(x, cos, sin, T, 0, B)
-        for layer, (st, cache, ws, ns) in zip(self.layers, kept):  # the decode state stays as it was
-            layer.state, layer.cache, layer.attn_ws, layer.n_splits = st, cache, ws, ns
-        return self._logits(x[:, -1])
+        return self._forward_only(idx)(-1)
+
+    @torch.no_grad()
+    def score(self, idx, temperature=1.0, n_top=0, positions=512):
+        """TokenLogprobs of idx [B, T]: token t's log probability given those before it, [B, T - 1]
+        (no caches kept); logits exist for `positions` positions at a time."""
+        logits = self._forward_only(idx)
+        parts = [token_logprobs(logits(slice(t, min(t + positions, idx.shape[1] - 1))),
+                                idx[:, t + 1:min(t + positions, idx.shape[1] - 1) + 1], temperature, n_top)
+                 for t in range(0, idx.shape[1] - 1, positions)]
+        return type(parts[0])(*(torch.cat(c, 1) for c in zip(*parts)))
 
     def _step_logits(self, tok):
         """One decode step on the device: every position-dependent value comes from self.pos,
@@ -196,10 +265,16 @@ class HybridLlama(nn.Module):
         dtype = self.embed.weight.dtype
         cos, sin = ang.cos().to(dtype), ang.sin().to(dtype)
         x = self.embed(tok[:, None])
+        if self.head is None:
+            for layer in self.layers:
+                x = layer.step(x, cos, sin, self.pos)
+            self.pos.add_(1)
+            return self._logits(x[:, -1])
+        d = None
         for layer in self.layers:
-            x = layer.step(x, cos, sin, self.pos)
+            d, x = layer.step_int8(d, x, cos, sin, self.pos)
         self.pos.add_(1)
-        return self._logits(x[:, -1])
+        return self.head(add_rms_norm_int8(d[:, -1], x[:, -1], self.norm.weight, self.norm.eps)[0])
 
     def _advance(self, n):
         self.n_tokens += n
@@ -220,6 +295,14 @@ class HybridLlama(nn.Module):
     def step(self, tok):
         """tok [B] -> next-token ids [B] (greedy)."""
         return self.step_logits(tok).argmax(-1)
+
+    @torch.no_grad()
+    def step_logprobs(self, tok, n_top=0, temperature=1.0):
+        """(next-token ids [B], their TokenLogprobs): a greedy step that answers with log
+        probabilities, entropies and n_top alternatives."""
+        logits = self.step_logits(tok)
+        nxt = logits.argmax(-1)
+        return nxt, token_logprobs(logits, nxt, temperature, n_top)
 
 
 class DecodeGraph:
