@@ -199,7 +199,9 @@ struct Shared {
 // G (rank + 1) / C), thread t those at t, t + kNT, ... of them, kBatch on their way at a time.
 template <typename T, int kNT>
 __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, const int C) {
-  constexpr int kBatch = 4, kWarps = kNT / 32;
+  // (with the next batch on its way: 8192 x 50257 bf16 takes 168 us in batches of one granule, 141
+  // of two, 148 of four, and 285 without)
+  constexpr int kBatch = 2, kWarps = kNT / 32;
   constexpr int kCandidates = kNT == 32 ? 256 : 1024;  // entries at or above the bound that are ranked at once
   __shared__ Shared sh;
   __shared__ Stat warp_stat[kWarps];
@@ -229,44 +231,69 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
   // ---- one pass: maximum, S, U, and the granule that holds the thread's first maximum
   Stat st = {-INFINITY, 0.f, 0.f};
   int best = g0 + tid;
-  for (int j = g0 + tid; j < g1; j += kBatch * kNT) {
-    uint4 v[kBatch];
-    float gm[kBatch];
+  const float2 c2 = make_float2(a.c, a.c);
+  auto absorb = [&](auto &v, int j) {  // granules j, j + kNT, ... of the thread
+    constexpr int n = sizeof(v) / sizeof(uint4);
+    float gm[n], bm = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-      if (j + b * kNT < g1) v[b] = view.load(j + b * kNT);
-    float bm = -INFINITY;
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      gm[b] = j + b * kNT < g1 ? granule_max<T>(v[b]) : -INFINITY;
+    for (int b = 0; b < n; ++b) {
+      gm[b] = granule_max<T>(v[b]);
       bm = fmaxf(bm, gm[b]);
     }
     if (bm > st.m) {
 #pragma unroll
-      for (int b = kBatch - 1; b >= 0; --b)
+      for (int b = n - 1; b >= 0; --b)
         if (gm[b] == bm) best = j + b * kNT;
       st.rebase(bm, a.c);
     }
     const float m = st.m == -INFINITY ? 0.f : st.m;
-    const float2 m2 = make_float2(-m, -m), c2 = make_float2(a.c, a.c);
+    const float2 m2 = make_float2(-m, -m);
     float2 s2 = make_float2(0.f, 0.f), u2 = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-      if (j + b * kNT < g1) {
-        float f[kPer<T>];
-        unpack<T>(v[b], f);
+    for (int b = 0; b < n; ++b) {
+      float f[kPer<T>];
+      unpack<T>(v[b], f);
 #pragma unroll
-        for (int k = 0; k < kPer<T>; k += 2) {
-          float2 d = __fmul2_rn(__fadd2_rn(make_float2(f[k], f[k + 1]), m2), c2);
-          const float2 e = make_float2(exp2_approx(d.x), exp2_approx(d.y));
-          d.x = fmaxf(d.x, -200.f);  // 2^-200 is 0 in fp32; -infinity times it would be NaN
-          d.y = fmaxf(d.y, -200.f);
-          s2 = __fadd2_rn(s2, e);
-          u2 = __ffma2_rn(e, d, u2);
-        }
+      for (int k = 0; k < kPer<T>; k += 2) {
+        float2 d = __fmul2_rn(__fadd2_rn(make_float2(f[k], f[k + 1]), m2), c2);
+        const float2 e = make_float2(exp2_approx(d.x), exp2_approx(d.y));
+        d.x = fmaxf(d.x, -200.f);  // 2^-200 is 0 in fp32; -infinity times it would be NaN
+        d.y = fmaxf(d.y, -200.f);
+        s2 = __fadd2_rn(s2, e);
+        u2 = __ffma2_rn(e, d, u2);
       }
+    }
     st.s += s2.x + s2.y;
     st.u += u2.x + u2.y;
+  };
+  // The row's whole granules; the next batch is on its way while this one is worked on.
+  const int whole0 = view.off ? 1 : 0, whole1 = (a.V + view.off) / kPer<T>;
+  const int w1 = min(g1, whole1);
+  int j = g0 + tid;
+  if (j < whole0) {  // (a first granule with some of the row: one thread's)
+    const uint4 v[1] = {view.load(j)};
+    absorb(v, j);
+    j += kNT;
+  }
+  const uint4 *base = reinterpret_cast<const uint4 *>(view.row - view.off);
+  uint4 v[kBatch];
+  if (j + (kBatch - 1) * kNT < w1) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) v[b] = __ldg(base + j + b * kNT);
+    for (; j + (2 * kBatch - 1) * kNT < w1; j += kBatch * kNT) {
+      uint4 next[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) next[b] = __ldg(base + j + (kBatch + b) * kNT);
+      absorb(v, j);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) v[b] = next[b];
+    }
+    absorb(v, j);
+    j += kBatch * kNT;
+  }
+  for (; j < g1; j += kNT) {
+    const uint4 one[1] = {j < w1 ? __ldg(base + j) : view.load(j)};
+    absorb(one, j);
   }
   const float thread_max = st.m;
   st.join_warp(a.c);
@@ -306,24 +333,29 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
     }
     __syncthreads();
     const unsigned long long t = tau;
-    if (mine && mine >= t) owner[atomicAdd(&n_owner, 1)] = tid;
-    __syncthreads();
-    const int owners = n_owner;
-    for (int w = warp; w < owners; w += kWarps) {
-      for (int j = g0 + owner[w] + lane * kNT; j < g1; j += 32 * kNT) {
-        const uint4 v = view.load(j);
-        float f[kPer<T>];
-        unpack<T>(v, f);
+    auto offer = [&](int j) {  // a granule's entries that reach the bound
+      const uint4 v = view.load(j);
+      float f[kPer<T>];
+      unpack<T>(v, f);
 #pragma unroll
-        for (int k = 0; k < kPer<T>; ++k) {
-          const int e = view.first(j) + k;
-          const unsigned long long key = order_key(f[k], e);
-          if (key >= t && e >= 0 && e < a.V) {
-            const int n = atomicAdd(&n_cand, 1);
-            if (n < kCandidates) cand[n] = key;
-          }
+      for (int k = 0; k < kPer<T>; ++k) {
+        const int e = view.first(j) + k;
+        const unsigned long long key = order_key(f[k], e);
+        if (key >= t && e >= 0 && e < a.V) {
+          const int n = atomicAdd(&n_cand, 1);
+          if (n < kCandidates) cand[n] = key;
         }
       }
+    };
+    if (kNT == 32 && g1 - g0 <= 8 * kNT) {  // each lane its own few granules
+      if (mine && mine >= t)
+        for (int j = g0 + tid; j < g1; j += kNT) offer(j);
+    } else {  // a warp at a time for each thread that has some
+      if (mine && mine >= t) owner[atomicAdd(&n_owner, 1)] = tid;
+      __syncthreads();
+      const int owners = n_owner;
+      for (int w = warp; w < owners; w += kWarps)
+        for (int j = g0 + owner[w] + lane * kNT; j < g1; j += 32 * kNT) offer(j);
     }
     __syncthreads();
     const int n = n_cand;
@@ -335,6 +367,7 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
       for (int i = tid; i < n; i += kNT) {
         const unsigned long long k = cand[i];
         int above = 0;
+#pragma unroll 8
         for (int q = 0; q < n; ++q) above += cand[q] > k;
         if (above < a.n_top) out[above] = k;
       }
@@ -411,6 +444,7 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
     int place = i;
     if (C > 1) {
       place = 0;
+#pragma unroll 8
       for (int q = 0; q < n; ++q) place += sh.top[q] > k;
     }
     if (k && place < a.n_top) {
@@ -454,7 +488,7 @@ struct RowGrad {
 // accesses but at a row's ends.  Grid (rows, shares of a row).
 template <typename T, bool ENTROPY, int kNT>
 __global__ void __launch_bounds__(kNT) logprobs_bwd_kernel(const BwdArgs a) {
-  constexpr int kBatch = 2;  // (four leave room for fewer blocks: 8192 x 50257 bf16 343 us against 313)
+  constexpr int kBatch = 2;  // (8192 x 50257 bf16: 272 us with one, 261 with two, 254 with four, which lose on short rows)
   const long long row = blockIdx.x;
   const RowGrad g(a, row);
   const RowView<T> view(a.logits, row, a.stride, a.rows, a.V);
@@ -463,66 +497,95 @@ __global__ void __launch_bounds__(kNT) logprobs_bwd_kernel(const BwdArgs a) {
   const int g0 = (int)((long long)G * blockIdx.y / C), g1 = (int)((long long)G * (blockIdx.y + 1) / C);
   const float2 m2 = make_float2(-g.lm, -g.lm), c2 = make_float2(a.c, a.c), s2 = make_float2(-g.log_s, -g.log_s);
   const float2 A2 = make_float2(g.A, g.A), B2 = make_float2(g.B, g.B);
-  // the granule and place of the token's entry
-  const bool has = g.token >= 0 && g.token < a.V;
-  const int token_at = has ? (int)g.token + view.off : -1;
-  for (int j = g0 + threadIdx.x; j < g1; j += kBatch * kNT) {
-    uint4 v[kBatch];
-    if (!g.zero) {
+  // where the token's entry lies, counted from the first granule's start
+  const int token_at = g.token >= 0 && g.token < a.V ? (int)g.token + view.off : -1;
+
+  auto gradient = [&](const uint4 &v, int j, float(&f)[kPer<T>]) {
+    unpack<T>(v, f);
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b)
-        if (j + b * kNT < g1) v[b] = view.load(j + b * kNT);
-    }
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int jj = j + b * kNT;
-      if (jj >= g1) continue;
-      float f[kPer<T>];
-      if (g.zero) {
-#pragma unroll
-        for (int k = 0; k < kPer<T>; ++k) f[k] = 0.f;
-      } else {
-        unpack<T>(v[b], f);
-#pragma unroll
-        for (int k = 0; k < kPer<T>; k += 2) {
-          float2 q = __ffma2_rn(__fadd2_rn(make_float2(f[k], f[k + 1]), m2), c2, s2);  // log2 p
-          const float2 p = make_float2(exp2_approx(q.x), exp2_approx(q.y));
-          float2 w = A2;
-          if (ENTROPY) {
-            q.x = fmaxf(q.x, -200.f);  // p is 0 there, and -infinity times it would be NaN
-            q.y = fmaxf(q.y, -200.f);
-            w = __ffma2_rn(B2, q, A2);
-          }
-          w = __fmul2_rn(p, w);
-          f[k] = w.x, f[k + 1] = w.y;
-        }
-        if (token_at >= jj * kPer<T> && token_at < (jj + 1) * kPer<T>) {
-#pragma unroll
-          for (int k = 0; k < kPer<T>; ++k)
-            if (token_at == jj * kPer<T> + k) f[k] += g.one;
-        }
+    for (int k = 0; k < kPer<T>; k += 2) {
+      float2 q = __ffma2_rn(__fadd2_rn(make_float2(f[k], f[k + 1]), m2), c2, s2);  // log2 p
+      const float2 p = make_float2(exp2_approx(q.x), exp2_approx(q.y));
+      float2 w = A2;
+      if (ENTROPY) {
+        q.x = fmaxf(q.x, -200.f);  // p is 0 there, and -infinity times it would be NaN
+        q.y = fmaxf(q.y, -200.f);
+        w = __ffma2_rn(B2, q, A2);
       }
-      const int e = view.first(jj);
-      if (e >= 0 && e + kPer<T> <= a.V) {
-        uint4 o;
-        if constexpr (sizeof(T) == 2) {
-          uint32_t *u = reinterpret_cast<uint32_t *>(&o);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
-            u[k] = *reinterpret_cast<const uint32_t *>(&h);
-          }
-        } else {
-          o = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-        }
-        *reinterpret_cast<uint4 *>(d + e) = o;
-      } else {
-#pragma unroll
-        for (int k = 0; k < kPer<T>; ++k)
-          if (e + k >= 0 && e + k < a.V) d[e + k] = from_f<T>(f[k]);
-      }
+      w = __fmul2_rn(p, w);
+      f[k] = w.x, f[k + 1] = w.y;
     }
+    if (token_at >= j * kPer<T> && token_at < (j + 1) * kPer<T>) {
+#pragma unroll
+      for (int k = 0; k < kPer<T>; ++k)
+        if (token_at == j * kPer<T> + k) f[k] += g.one;
+    }
+  };
+  const uint4 *from = reinterpret_cast<const uint4 *>(view.row - view.off);
+  uint4 *to = reinterpret_cast<uint4 *>(d - view.off);
+  auto whole = [&](const uint4 &v, int j) {
+    float f[kPer<T>];
+    gradient(v, j, f);
+    uint4 o;
+    if constexpr (sizeof(T) == 2) {
+      uint32_t u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
+        u[k] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+      o = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+      o = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+    to[j] = o;
+  };
+  auto part = [&](int j) {  // a granule that the row has some of
+    float f[kPer<T>];
+    if (g.zero) {
+#pragma unroll
+      for (int k = 0; k < kPer<T>; ++k) f[k] = 0.f;
+    } else {
+      gradient(view.load(j), j, f);
+    }
+    const int e = view.first(j);
+#pragma unroll
+    for (int k = 0; k < kPer<T>; ++k)
+      if (e + k >= 0 && e + k < a.V) d[e + k] = from_f<T>(f[k]);
+  };
+
+  const int whole0 = view.off ? 1 : 0, w1 = min(g1, (a.V + view.off) / kPer<T>);
+  int j = g0 + threadIdx.x;
+  if (j < whole0) {
+    part(j);
+    j += kNT;
   }
+  if (g.zero) {
+    for (; j < w1; j += kNT) to[j] = make_uint4(0, 0, 0, 0);
+  } else if (j + (kBatch - 1) * kNT < w1) {
+    // the next batch is on its way while this one is worked on
+    uint4 v[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) v[b] = __ldg(from + j + b * kNT);
+    for (; j + (2 * kBatch - 1) * kNT < w1; j += kBatch * kNT) {
+      uint4 next[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) next[b] = __ldg(from + j + (kBatch + b) * kNT);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        whole(v[b], j + b * kNT);
+        v[b] = next[b];
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) whole(v[b], j + b * kNT);
+    j += kBatch * kNT;
+  }
+  for (; j < g1; j += kNT)
+    if (j < w1)
+      whole(__ldg(from + j), j);
+    else
+      part(j);
 }
 
 // Any layout, one value at a time.
