@@ -21,6 +21,13 @@ __device__ __forceinline__ float corner_sign(int r, int p, int P) {
   return ((r >> (P - 1 - p)) & 1) ? 1.f : -1.f;
 }
 
+// For kernels launched by launch_early(): nothing of what earlier kernels on the stream read or
+// write is touched before wait_for_predecessor(), which returns once they are done.  After
+// let_successor_start() (by a thread of every block, or at its end) the next such kernel's blocks
+// may take what room is left on the SMs: a kernel calls it once it holds all it needs.
+__device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_successor_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __host__ __device__ __forceinline__ size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 }  // namespace race

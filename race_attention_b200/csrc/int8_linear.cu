@@ -203,15 +203,18 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__
     ctl[1] = (int)a.wait_limit;
     bad = 0;
     tc::fence_mbar_init();
+    race::wait_for_predecessor();
     while (issued < wanted && issued < C::kStages) load_next();
   }
   if (warp == 1) tc::tmem_alloc(&tmem_slot, C::kCols);
+  race::wait_for_predecessor();
   for (int t = (int)threadIdx.x - 64; t < tokens; t += kThreads - 64)
-    if (t >= 0) xs[t] = __ldg(a.xs + m0 + t);
+    if (t >= 0) xs[t] = a.xs[m0 + t];
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  race::let_successor_start();  // (this block has its shared memory and TMEM)
   if (S > 1) cluster_arrive();  // this block runs, and its `bad` is clear
 
   if (warp == 0) {
@@ -287,8 +290,8 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int nn = min(n + j, a.N - 1);
-      ws[j] = __ldg(a.ws + nn);
-      bias[j] = a.bias ? __ldg(a.bias + nn) : 0.f;
+      ws[j] = a.ws[nn];
+      bias[j] = a.bias ? a.bias[nn] : 0.f;
     }
     T *y = static_cast<T *>(a.y) + (long long)m0 * a.N + n;
 #pragma unroll 4
@@ -471,11 +474,11 @@ pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUte
       {
         static_assert(kPairN == 32 * kOutWarps, "one channel per epilogue thread");
         const int n = min(n0 + et, a.N - 1);
-        scale[et] = __ldg(a.ws + n);
-        bias[et] = a.bias ? __ldg(a.bias + n) : 0.f;
+        scale[et] = a.ws[n];
+        bias[et] = a.bias ? a.bias[n] : 0.f;
       }
       const int m = m0 + lane;
-      const float xs = m < a.M ? __ldg(a.xs + m) : 0.f;
+      const float xs = m < a.M ? a.xs[m] : 0.f;
       tc::named_bar_sync(1, 32 * kOutWarps);
       const bool ok = tc::warp_all(!*abort && tc::mbar_wait(&acc_full[buf], use & 1, abort));
       tc::tc_fence_after();
@@ -597,18 +600,8 @@ int launch_split(const CUtensorMap &mx, const CUtensorMap &mw, const Args &a, cu
   int S = 1;
   constexpr int kMost = BT <= 64 ? kMaxSplit : kMaxSplit / 2;
   while (S < kMost && 2LL * S * n_tiles * m_tiles <= room && a.k_steps >= 4 * S) S *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(n_tiles * S), (unsigned)m_tiles);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Split<BT>::kBytes;
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)S;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = S > 1;
-  e = cudaLaunchKernelEx(&cfg, split_kernel<T, BT>, mx, mw, a, S);
+  e = race::launch_early(split_kernel<T, BT>, dim3((unsigned)(n_tiles * S), (unsigned)m_tiles), dim3(kThreads),
+                         Split<BT>::kBytes, s, (unsigned)S, mx, mw, a, S);
   if (e != cudaSuccess) return cuda_err("int8_linear", e);
   return race::launched("int8_linear");
 }

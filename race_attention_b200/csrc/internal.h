@@ -40,6 +40,27 @@ inline int cuda_err(const char *what, cudaError_t e) {
   snprintf(buf, sizeof(buf), "%s: %s", what, cudaGetErrorString(e));
   return report_error(RACE_ERR_CUDA, buf);
 }
+// Launch of a kernel that starts with wait_for_predecessor(): with the stream's previous kernel
+// still running (once all of its blocks are past let_successor_start(), or done), so that its
+// launch and whatever it does before that call overlap it.
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, unsigned cluster,
+                         const A &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
 // After a launch: counts it, and turns its error into a status.
 inline int launched(const char *what) {
   note_launch();

@@ -114,11 +114,11 @@ struct RowView {
     const T *g = row + e;
     uint4 v;
     if (e >= 0 && e + kPer<T> <= V) {
-      v = __ldg(reinterpret_cast<const uint4 *>(g));
+      v = *reinterpret_cast<const uint4 *>(g);
     } else {
       uint32_t u[4];
       const bool whole = g >= begin && g + kPer<T> <= end;
-      if (whole) v = __ldg(reinterpret_cast<const uint4 *>(g));
+      if (whole) v = *reinterpret_cast<const uint4 *>(g);
       u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
 #pragma unroll
       for (int k = 0; k < kPer<T>; ++k) {
@@ -126,13 +126,13 @@ struct RowView {
         if constexpr (sizeof(T) == 2) {
           const int s = 16 * (k & 1);
           uint32_t x = 0xff80u;
-          if (has) x = whole ? (u[k / 2] >> s) & 0xffffu : (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(g) + k);
+          if (has) x = whole ? (u[k / 2] >> s) & 0xffffu : (uint32_t)reinterpret_cast<const uint16_t *>(g)[k];
           u[k / 2] = (u[k / 2] & (0xffff0000u >> s)) | (x << s);
         } else {
           if (!has)
             u[k] = 0xff800000u;
           else if (!whole)
-            u[k] = __ldg(reinterpret_cast<const uint32_t *>(g) + k);
+            u[k] = reinterpret_cast<const uint32_t *>(g)[k];
         }
       }
       v = make_uint4(u[0], u[1], u[2], u[3]);
@@ -210,6 +210,8 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = blockIdx.x % C;
   const long long row = blockIdx.x / C;
+  race::wait_for_predecessor();
+  race::let_successor_start();
   const long long token = a.tokens[row];
   if (token == a.ignore) {  // the whole cluster leaves
     if (rank == 0 && tid == 0) {
@@ -279,11 +281,11 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
   uint4 v[kBatch];
   if (j + (kBatch - 1) * kNT < w1) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) v[b] = __ldg(base + j + b * kNT);
+    for (int b = 0; b < kBatch; ++b) v[b] = base[j + b * kNT];
     for (; j + (2 * kBatch - 1) * kNT < w1; j += kBatch * kNT) {
       uint4 next[kBatch];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) next[b] = __ldg(base + j + (kBatch + b) * kNT);
+      for (int b = 0; b < kBatch; ++b) next[b] = base[j + (kBatch + b) * kNT];
       absorb(v, j);
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) v[b] = next[b];
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
     j += kBatch * kNT;
   }
   for (; j < g1; j += kNT) {
-    const uint4 one[1] = {j < w1 ? __ldg(base + j) : view.load(j)};
+    const uint4 one[1] = {j < w1 ? base[j] : view.load(j)};
     absorb(one, j);
   }
   const float thread_max = st.m;
@@ -489,6 +491,8 @@ struct RowGrad {
 template <typename T, bool ENTROPY, int kNT>
 __global__ void __launch_bounds__(kNT) logprobs_bwd_kernel(const BwdArgs a) {
   constexpr int kBatch = 2;  // (8192 x 50257 bf16: 272 us with one, 261 with two, 254 with four, which lose on short rows)
+  race::wait_for_predecessor();
+  race::let_successor_start();
   const long long row = blockIdx.x;
   const RowGrad g(a, row);
   const RowView<T> view(a.logits, row, a.stride, a.rows, a.V);
@@ -566,11 +570,11 @@ __global__ void __launch_bounds__(kNT) logprobs_bwd_kernel(const BwdArgs a) {
     // the next batch is on its way while this one is worked on
     uint4 v[kBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) v[b] = __ldg(from + j + b * kNT);
+    for (int b = 0; b < kBatch; ++b) v[b] = from[j + b * kNT];
     for (; j + (2 * kBatch - 1) * kNT < w1; j += kBatch * kNT) {
       uint4 next[kBatch];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) next[b] = __ldg(from + j + (kBatch + b) * kNT);
+      for (int b = 0; b < kBatch; ++b) next[b] = from[j + (kBatch + b) * kNT];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         whole(v[b], j + b * kNT);
@@ -583,7 +587,7 @@ __global__ void __launch_bounds__(kNT) logprobs_bwd_kernel(const BwdArgs a) {
   }
   for (; j < g1; j += kNT)
     if (j < w1)
-      whole(__ldg(from + j), j);
+      whole(from[j], j);
     else
       part(j);
 }
@@ -591,6 +595,8 @@ __global__ void __launch_bounds__(kNT) logprobs_bwd_kernel(const BwdArgs a) {
 // Any layout, one value at a time.
 template <typename T, int kNT>
 __global__ void __launch_bounds__(kNT) logprobs_bwd_loop_kernel(const BwdArgs a) {
+  race::wait_for_predecessor();
+  race::let_successor_start();
   const long long row = blockIdx.x;
   const RowGrad g(a, row);
   const T *l = static_cast<const T *>(a.logits) + row * a.stride;
@@ -613,17 +619,8 @@ int launch_fwd_threads(const FwdArgs &a, cudaStream_t s) {
   int C = 1;
   if (kNT == 256)
     while (C < kMaxCluster && a.rows * C * 2 <= 4 * 148 && a.V >= 2 * C * kNT * kPer<T>) C *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.rows * C));
-  cfg.blockDim = dim3(kNT);
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)C;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = C > 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, kNT>, a, C);
+  const cudaError_t e =
+      race::launch_early(logprobs_fwd_kernel<T, kNT>, dim3((unsigned)(a.rows * C)), dim3(kNT), 0, s, (unsigned)C, a, C);
   if (e != cudaSuccess) return race::cuda_err("token_logprobs_fwd", e);
   return launched("token_logprobs_fwd");
 }
@@ -647,11 +644,11 @@ int launch_bwd_threads(const BwdArgs &a, cudaStream_t s) {
   const uintptr_t l = reinterpret_cast<uintptr_t>(a.logits), d = reinterpret_cast<uintptr_t>(a.dlogits);
   if (((l ^ d) & 15) == 0 && (a.stride - a.V) % kPer<T> == 0) {
     if (a.g_entropy)
-      logprobs_bwd_kernel<T, true, kNT><<<grid, kNT, 0, s>>>(a);
+      race::launch_early(logprobs_bwd_kernel<T, true, kNT>, grid, dim3(kNT), 0, s, 1, a);
     else
-      logprobs_bwd_kernel<T, false, kNT><<<grid, kNT, 0, s>>>(a);
+      race::launch_early(logprobs_bwd_kernel<T, false, kNT>, grid, dim3(kNT), 0, s, 1, a);
   } else {
-    logprobs_bwd_loop_kernel<T, kNT><<<grid, kNT, 0, s>>>(a);
+    race::launch_early(logprobs_bwd_loop_kernel<T, kNT>, grid, dim3(kNT), 0, s, 1, a);
   }
   return launched("token_logprobs_bwd");
 }

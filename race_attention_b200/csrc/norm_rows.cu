@@ -110,7 +110,16 @@ constexpr int kWords = 2 * (int)sizeof(T);  // 32-bit words of 8 values
 template <typename T>
 constexpr int kPerG = 16 / (int)sizeof(T);  // values per 16-byte granule
 
-__device__ __forceinline__ uint4 ldg16(const void *p) { return __ldg(static_cast<const uint4 *>(p)); }
+// A load of inputs.  Those of a kernel that is launched early are not constant over its run (its
+// predecessor may still write them), so the read-only path, whose loads a compiler may move, is
+// for the others.
+template <bool CONST, typename V>
+__device__ __forceinline__ V input(const V *p) {
+  if constexpr (CONST)
+    return __ldg(p);
+  else
+    return *p;
+}
 
 template <typename T>
 __device__ __forceinline__ int misalign(const T *p) {  // values past a granule's start
@@ -175,7 +184,7 @@ __device__ __forceinline__ void floats_to_words(const float *f, uint32_t *u) {
 
 // Eight values as they came from memory, unpacked where they are used so that many are in
 // flight at once.
-template <typename T, int LAYOUT>
+template <typename T, int LAYOUT, bool CONST = false>
 struct Vec8 {
   static constexpr int N = kWords<T> + (LAYOUT == kShifted ? 4 : 0);
   uint32_t c[N];
@@ -185,7 +194,7 @@ struct Vec8 {
   __device__ __forceinline__ void granules(const T *g) {
 #pragma unroll
     for (int i = 0; i < M; i += 4) {
-      const uint4 v = ldg16(reinterpret_cast<const uint32_t *>(g) + i);
+      const uint4 v = input<CONST>(reinterpret_cast<const uint4 *>(g) + i / 4);
       c[i] = v.x, c[i + 1] = v.y, c[i + 2] = v.z, c[i + 3] = v.w;
     }
   }
@@ -194,9 +203,9 @@ struct Vec8 {
     for (int k = 0; k < 8; ++k)
       if (e + k >= 0 && e + k < K) {
         if constexpr (sizeof(T) == 2)
-          c[k / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(p) + e + k) << (16 * (k & 1));
+          c[k / 2] |= (uint32_t)input<CONST>(reinterpret_cast<const uint16_t *>(p) + e + k) << (16 * (k & 1));
         else
-          c[k] = __ldg(reinterpret_cast<const uint32_t *>(p) + e + k);
+          c[k] = input<CONST>(reinterpret_cast<const uint32_t *>(p) + e + k);
       }
   }
   // Values e .. e + 7 of the row p of K values, of a tensor whose values lie in [begin, end).
@@ -261,12 +270,12 @@ __device__ __forceinline__ void weights8(const void *w, int w_bf16, bool whole, 
     uint32_t u[8];
     const uint32_t *g = w_bf16 ? reinterpret_cast<const uint32_t *>(static_cast<const __nv_bfloat16 *>(w) + e)
                                : reinterpret_cast<const uint32_t *>(static_cast<const float *>(w) + e);
-    const uint4 v = ldg16(g);
+    const uint4 v = *reinterpret_cast<const uint4 *>(g);
     u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
     if (w_bf16) {
       words_to_floats<__nv_bfloat16>(u, f);
     } else {
-      const uint4 v2 = ldg16(g + 4);
+      const uint4 v2 = *reinterpret_cast<const uint4 *>(g + 4);
       u[4] = v2.x, u[5] = v2.y, u[6] = v2.z, u[7] = v2.w;
       words_to_floats<float>(u, f);
     }
@@ -369,6 +378,8 @@ __global__ void __launch_bounds__(row_block(G)) row_kernel(const RowArgs a) {
   __shared__ uint2 line[LAYOUT == kSkewed && MODE != kNorm ? kPer * (G * VPT + 1) : 1];
   constexpr bool kTwo = MODE != kQuantInt8;  // a second input: the residual, or SwiGLU's other half
   constexpr bool kIsNorm = MODE == kNorm || MODE == kNormInt8;
+  race::wait_for_predecessor();
+  race::let_successor_start();
   const int size = group_size<G>(), tid = G == 32 ? threadIdx.x % 32 : threadIdx.x, K = a.K;
   const long long first = (long long)blockIdx.x * kPer + (G == 32 ? threadIdx.x / 32 : 0);
   const long long step = LAYOUT == kSkewed ? (long long)gridDim.x * kPer : a.rows;
@@ -558,7 +569,7 @@ __global__ void __launch_bounds__(row_block(G), G == 320 ? 2 : 512 / row_block(G
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
 
   struct Row {
-    Vec8<T, LAYOUT> dy[VPT], h[VPT], dh[VPT];
+    Vec8<T, LAYOUT, true> dy[VPT], h[VPT], dh[VPT];
     float rstd;
   };
   auto load = [&](Row &s, long long row) {
@@ -633,6 +644,7 @@ __global__ void __launch_bounds__(row_block(G), G == 320 ? 2 : 512 / row_block(G
 // dw[k] = sum of the blocks' partial sums, in a fixed order.
 __global__ void __launch_bounds__(1024) dw_sum_kernel(const float *part, int n, int K, void *dw, int w_bf16) {
   __shared__ float red[32][33];
+  race::wait_for_predecessor();
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, k = blockIdx.x * 32 + lane;
   float s = 0.f;
   if (k < K) {
@@ -660,9 +672,11 @@ __global__ void __launch_bounds__(1024) dw_sum_kernel(const float *part, int n, 
 template <typename T>
 __global__ void __launch_bounds__(256) dequant_kernel(const int8_t *q_rows, long long q_stride, const float *scale, T *out,
                                                       long long rows, int K, bool q_vec) {
+  race::wait_for_predecessor();
+  race::let_successor_start();
   const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= rows) return;
-  const float s = __ldg(scale + row);
+  const float s = scale[row];
   const int8_t *q = q_rows + row * q_stride;
   T *o = out + row * K;
   const int off = misalign(o);
@@ -670,9 +684,9 @@ __global__ void __launch_bounds__(256) dequant_kernel(const int8_t *q_rows, long
     const int w = e & ~7, shift = 8 * (e & 3);  // the word that holds byte e
     uint32_t lo = 0, hi = 0;
     if (q_vec && w >= 0 && w + (off ? 16 : 8) <= K) {
-      const uint2 a = __ldg(reinterpret_cast<const uint2 *>(q + w));
+      const uint2 a = *reinterpret_cast<const uint2 *>(q + w);
       uint2 b = make_uint2(0, 0);
-      if (off) b = __ldg(reinterpret_cast<const uint2 *>(q + w + 8));
+      if (off) b = *reinterpret_cast<const uint2 *>(q + w + 8);
       const bool half = e & 4;
       const uint32_t c0 = half ? a.y : a.x, c1 = half ? b.x : a.y, c2 = half ? b.y : b.x;
       lo = __funnelshift_r(c0, c1, shift);
@@ -681,7 +695,7 @@ __global__ void __launch_bounds__(256) dequant_kernel(const int8_t *q_rows, long
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         if (e + k >= 0 && e + k < K) {
-          const uint32_t v = (uint32_t)(uint8_t)__ldg(q + e + k) << (8 * (k & 3));
+          const uint32_t v = (uint32_t)(uint8_t)q[e + k] << (8 * (k & 3));
           if (k < 4)
             lo |= v;
           else
@@ -730,7 +744,7 @@ void launch_row_kernel(const RowArgs &a, int vectors, cudaStream_t s) {
     const long long most = 148 * (2048 / threads) / 8 * 8;
     blocks = blocks < most ? (blocks + 7) / 8 * 8 : most;
   }
-  row_kernel<T, MODE, G, VPT, LAYOUT><<<(unsigned)blocks, threads, 0, s>>>(a);
+  race::launch_early(row_kernel<T, MODE, G, VPT, LAYOUT>, dim3((unsigned)blocks), dim3(threads), 0, s, 1, a);
 }
 
 // Threads per row.  A warp up to 1024 values: no barriers, all of a row's loads in flight at
@@ -744,7 +758,7 @@ void launch_width(const RowArgs &a, cudaStream_t s) {
   const int n = (a.K + (LAYOUT == kSkewed ? 7 : 0) + 7) / 8;  // vectors, whatever the offset
   const bool few = a.rows < 1184;  // eight blocks on each SM of a B200
   if (n <= 32) return launch_row_kernel<T, MODE, 32, 1, LAYOUT>(a, n, s);
-  if (n <= 256 && few) return launch_row_kernel<T, MODE, 256, 1, LAYOUT>(a, n, s);
+  if (n <= 512 && few) return launch_row_kernel<T, MODE, 512, 1, LAYOUT>(a, n, s);
   if (n <= 64) return launch_row_kernel<T, MODE, 32, 2, LAYOUT>(a, n, s);
   if (n <= 96) return launch_row_kernel<T, MODE, 32, 3, LAYOUT>(a, n, s);
   if (n <= 128) return launch_row_kernel<T, MODE, 32, 4, LAYOUT>(a, n, s);
@@ -905,9 +919,11 @@ int race_dequant_int8(const int8_t *q, int64_t q_stride, const float *scale, voi
   const unsigned grid = (unsigned)((rows + block.y - 1) / block.y);
   const bool q_vec = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)q_stride) & 7) == 0;
   if (dtype == RACE_BF16)
-    dequant_kernel<<<grid, block, 0, s>>>(q, q_stride, scale, static_cast<__nv_bfloat16 *>(out), rows, (int)K, q_vec);
+    race::launch_early(dequant_kernel<__nv_bfloat16>, dim3(grid), block, 0, s, 1, q, q_stride, scale,
+                       static_cast<__nv_bfloat16 *>(out), rows, (int)K, q_vec);
   else
-    dequant_kernel<<<grid, block, 0, s>>>(q, q_stride, scale, static_cast<float *>(out), rows, (int)K, q_vec);
+    race::launch_early(dequant_kernel<float>, dim3(grid), block, 0, s, 1, q, q_stride, scale, static_cast<float *>(out), rows,
+                       (int)K, q_vec);
   return launched("dequant_int8");
 }
 
@@ -934,7 +950,8 @@ int race_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float
     launch_bwd<float>(a, blocks, s);
   if (const int rc = launched("rms_norm_bwd")) return rc;
   if (!dw) return RACE_OK;
-  dw_sum_kernel<<<(unsigned)((K + 31) / 32), 1024, 0, s>>>(a.part, blocks, (int)K, dw, weight_dtype == RACE_BF16);
+  race::launch_early(dw_sum_kernel, dim3((unsigned)((K + 31) / 32)), dim3(1024), 0, s, 1, a.part, blocks, (int)K, dw,
+                     (int)(weight_dtype == RACE_BF16));
   return launched("rms_norm_bwd dw");
 }
 
