@@ -264,24 +264,44 @@ __device__ __forceinline__ void store8(T *p, int e, int K, const float *f) {
   }
 }
 
-// weights e .. e + 7 (1 where there are none); `whole`: they are a vector from a granule on
-__device__ __forceinline__ void weights8(const void *w, int w_bf16, bool whole, int e, int K, float *f) {
-  if (w && whole) {
-    uint32_t u[8];
-    const uint32_t *g = w_bf16 ? reinterpret_cast<const uint32_t *>(static_cast<const __nv_bfloat16 *>(w) + e)
-                               : reinterpret_cast<const uint32_t *>(static_cast<const float *>(w) + e);
-    const uint4 v = *reinterpret_cast<const uint4 *>(g);
-    u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
-    if (w_bf16) {
-      words_to_floats<__nv_bfloat16>(u, f);
-    } else {
-      const uint4 v2 = *reinterpret_cast<const uint4 *>(g + 4);
-      u[4] = v2.x, u[5] = v2.y, u[6] = v2.z, u[7] = v2.w;
-      words_to_floats<float>(u, f);
+// weights e .. e + 7 (1 where there are none), put together from the granules that hold them;
+// ALIGNED: they are a vector's, from a granule on
+template <bool ALIGNED, typename W>
+__device__ __forceinline__ void weights8_of(const W *w, int e, int K, float *f) {
+  constexpr int N = kWords<W> + 4;
+  const W *p = w + e;
+  const int off = ALIGNED ? 0 : misalign(p);
+  const W *g = p - off;
+  uint32_t c[N];
+  if (ALIGNED ? e < K : off == 0 && e >= 0 && e + 8 <= K) {
+#pragma unroll
+    for (int i = 0; i < N - 4; i += 4) {
+      const uint4 v = reinterpret_cast<const uint4 *>(g)[i / 4];
+      c[i] = v.x, c[i + 1] = v.y, c[i + 2] = v.z, c[i + 3] = v.w;
     }
+    words_to_floats<W>(c, f);
+  } else if (!ALIGNED && g >= w && g + N * 4 / (int)sizeof(W) <= w + K) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 v = reinterpret_cast<const uint4 *>(g)[i / 4];
+      c[i] = v.x, c[i + 1] = v.y, c[i + 2] = v.z, c[i + 3] = v.w;
+    }
+    shift_down<W>(c, off);
+    words_to_floats<W>(c, f);
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = w && e + k >= 0 && e + k < K ? weight_at(w, w_bf16, e + k) : 1.f;
+    for (int k = 0; k < 8; ++k) f[k] = e + k >= 0 && e + k < K ? to_f<W>(w[e + k]) : 1.f;
+  }
+}
+template <bool ALIGNED>
+__device__ __forceinline__ void weights8(const void *w, int w_bf16, int e, int K, float *f) {
+  if (!w) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = 1.f;
+  } else if (w_bf16) {
+    weights8_of<ALIGNED>(static_cast<const __nv_bfloat16 *>(w), e, K, f);
+  } else {
+    weights8_of<ALIGNED>(static_cast<const float *>(w), e, K, f);
   }
 }
 
@@ -388,7 +408,7 @@ __global__ void __launch_bounds__(row_block(G)) row_kernel(const RowArgs a) {
   float w[kIsNorm && LAYOUT == kSkewed ? VPT * 8 : 1];
   if constexpr (kIsNorm && LAYOUT == kSkewed) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) weights8(a.w, a.w_bf16, false, at(i), K, w + 8 * i);
+    for (int i = 0; i < VPT; ++i) weights8<false>(a.w, a.w_bf16, at(i), K, w + 8 * i);
   }
   // the tensors' extents
   const T *x_begin = static_cast<const T *>(a.x), *x_end = x_begin + (a.rows - 1) * a.x_stride + (MODE == kSwigluInt8 ? 2 : 1) * (long long)K;
@@ -431,7 +451,7 @@ __global__ void __launch_bounds__(row_block(G)) row_kernel(const RowArgs a) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         float u[8];
-        if (LAYOUT != kSkewed) weights8(a.w, a.w_bf16, LAYOUT == kAligned && at(i) < K, at(i), K, u);
+        if (LAYOUT != kSkewed) weights8<LAYOUT == kAligned>(a.w, a.w_bf16, at(i), K, u);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[8 * i + j] = v[8 * i + j] * rstd * (LAYOUT == kSkewed ? w[kIsNorm && LAYOUT == kSkewed ? 8 * i + j : 0] : u[j]);
       }
@@ -564,7 +584,7 @@ __global__ void __launch_bounds__(row_block(G), G == 320 ? 2 : 512 / row_block(G
   auto at = [&](int i) { return (i * size + tid) * 8 - off; };  // where the thread's i-th vector starts
   float w[N], acc[N];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) weights8(a.w, a.w_bf16, false, at(i), K, w + 8 * i);
+  for (int i = 0; i < VPT; ++i) weights8<false>(a.w, a.w_bf16, at(i), K, w + 8 * i);
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
 
@@ -758,7 +778,7 @@ void launch_width(const RowArgs &a, cudaStream_t s) {
   const int n = (a.K + (LAYOUT == kSkewed ? 7 : 0) + 7) / 8;  // vectors, whatever the offset
   const bool few = a.rows < 1184;  // eight blocks on each SM of a B200
   if (n <= 32) return launch_row_kernel<T, MODE, 32, 1, LAYOUT>(a, n, s);
-  if (n <= 512 && few) return launch_row_kernel<T, MODE, 512, 1, LAYOUT>(a, n, s);
+  if (n <= 256 && few) return launch_row_kernel<T, MODE, 256, 1, LAYOUT>(a, n, s);
   if (n <= 64) return launch_row_kernel<T, MODE, 32, 2, LAYOUT>(a, n, s);
   if (n <= 96) return launch_row_kernel<T, MODE, 32, 3, LAYOUT>(a, n, s);
   if (n <= 128) return launch_row_kernel<T, MODE, 32, 4, LAYOUT>(a, n, s);
