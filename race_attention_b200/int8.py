@@ -62,21 +62,32 @@ def int8_linear(x: Int8Rows, w: Int8Rows, bias=None, dtype=torch.bfloat16):
 class Int8Linear(nn.Module):
     """A linear layer over 8-bit rows: weight rows and scales are buffers (inference only).
 
-    forward takes Int8Rows, or a float tensor which it quantises first."""
+    forward takes Int8Rows, or a float tensor which it quantises first.  The weight rows are held
+    padded to a multiple of 16 bytes, and the scales stay float32 when the module's type changes."""
 
     def __init__(self, weight, bias=None, dtype=torch.bfloat16):
         super().__init__()
-        rows = quant_int8(weight.detach())
-        self.register_buffer("q", rows.q)
-        self.register_buffer("scale", rows.scale)
-        self.register_buffer("bias", None if bias is None else bias.detach().float().contiguous())
         self.out_features, self.in_features = weight.shape
         self.dtype = dtype
+        rows = quant_int8(weight.detach())
+        q = rows.q
+        if self.in_features % 16:
+            q = nn.functional.pad(q, (0, -self.in_features % 16))
+        self.register_buffer("q", q)
+        self.register_buffer("scale", rows.scale)
+        self.register_buffer("bias", None if bias is None else bias.detach().float().contiguous())
 
     @classmethod
     def from_linear(cls, linear: nn.Linear):
         return cls(linear.weight, linear.bias, linear.weight.dtype)
 
+    def _apply(self, fn, *args, **kwargs):
+        held = self.scale, self.bias
+        super()._apply(fn, *args, **kwargs)
+        self.scale, self.bias = (None if t is None else t.to(self.q.device) for t in held)
+        return self
+
     def forward(self, x):
         rows = x if isinstance(x, Int8Rows) else quant_int8(x)
-        return int8_linear(rows, Int8Rows(self.q, self.scale), self.bias, self.dtype)
+        q = self.q if self.q.shape[1] == self.in_features else self.q[:, :self.in_features]
+        return int8_linear(rows, Int8Rows(q, self.scale), self.bias, self.dtype)

@@ -108,8 +108,34 @@ def test_linear_layer_from_a_float_one():
     want = torch.nn.functional.linear(x.double(), lin.weight.double(), lin.bias.double())
     y = layer(x)
     assert y.shape == want.shape and y.dtype == BF16
-    assert float((y.double() - want).norm() / want.norm()) < 0.02
+    assert float((y.double() - want).detach().norm() / want.detach().norm()) < 0.02
     assert set(layer.state_dict()) == {"q", "scale", "bias"}
+
+
+def test_linear_layer_of_odd_width_keeps_its_form_when_moved():
+    from race_attention_b200 import Int8Linear
+    torch.manual_seed(1)
+    layer = Int8Linear(torch.randn(65, 77, device="cuda"), torch.randn(65, device="cuda"), F32)
+    x = torch.randn(9, 77, device="cuda")
+    y = layer(x)
+    moved = layer.to(BF16).cpu().cuda()
+    assert moved.scale.dtype == F32 and moved.bias.dtype == F32 and moved.q.dtype == torch.int8
+    assert torch.equal(moved(x), y)
+    other = Int8Linear(torch.zeros(65, 77, device="cuda"), torch.zeros(65, device="cuda"), F32)
+    other.load_state_dict(layer.state_dict())
+    assert torch.equal(other(x), y)
+
+
+@pytest.mark.parametrize("M,N", [(66000, 33000), (33000, 66001)])
+def test_outputs_past_two_gigabytes(M, N):
+    """More than 2^31 outputs: the last rows and columns are where they belong."""
+    from race_attention_b200 import Int8Rows, int8_linear
+    g = _gen(31)
+    xq, xs = _rows(g, M, 64)
+    wq, ws = _rows(g, N, 64)
+    y = int8_linear(Int8Rows(xq, xs), Int8Rows(wq, ws))
+    for at in (slice(0, 2), slice(M - 300, M)):
+        _check(y[at], xq[at], xs[at], wq, ws, None, BF16)
 
 
 def test_other_stream_and_repeated_calls_give_the_same_bits():

@@ -118,6 +118,23 @@ def test_masks_and_rows_without_an_entry(V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [3, 1000, 70001])
+def test_rows_of_the_lowest_value_alone_are_uniform(V, dtype):
+    """A mask by the type's lowest value that leaves nothing: every entry is as probable."""
+    from race_attention_b200 import token_logprobs
+    logits = torch.full((3, V), torch.finfo(dtype).min, device="cuda", dtype=dtype, requires_grad=True)
+    tokens = torch.tensor([0, V // 2, V - 1], device="cuda")
+    got = token_logprobs(logits, tokens, n_top=2)
+    want = torch.full((3,), -math.log(V), device="cuda")
+    _near(got.logp, want, 2e-5, "logp")
+    _near(got.entropy, -want, 1e-4, "entropy")
+    assert torch.equal(got.top_ids.cpu(), torch.tensor([[0, 1]] * 3))
+    d, = torch.autograd.grad(got.logp.sum(), logits)
+    one = torch.zeros(3, V, device="cuda", dtype=torch.float64).scatter_(1, tokens[:, None], 1.0)
+    within(d, one - 1 / V, 1e-4 * (one + 1 / V), "dlogits")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows,V", [(1, 1), (2, 9), (5, 257), (3, 1000), (33, 8191), (6, 50257), (2, 131072), (700, 640)])
 def test_gradient(rows, V, dtype):
     from race_attention_b200 import token_logprobs

@@ -232,6 +232,29 @@ def test_int8_layouts():
     assert quant_int8(big[:0]).q.shape == (0, 5, 702)
 
 
+def test_rows_past_two_gigabytes():
+    """More than 2^31 values: the last rows, of aligned and of odd widths."""
+    from race_attention_b200 import add_rms_norm, add_rms_norm_int8, ops
+    g = _gen(14)
+    for rows, K in ((1_100_000, 2048), (1_150_001, 2047)):
+        x = torch.zeros(rows, K, device="cuda", dtype=BF16)
+        x[:2] = torch.randn(2, K, generator=g, device="cuda").to(BF16)
+        x[-9:] = torch.randn(9, K, generator=g, device="cuda").to(BF16)
+        ends = [0, 1] + list(range(rows - 9, rows))
+        y, h = add_rms_norm(x, x, None, eps=EPS)
+        want_h, want, rstd = _norm64(x[ends], x[ends], None)
+        assert torch.equal(h[ends], want_h)
+        _near(y[ends], want, BF16, what="y")
+        r8, _ = add_rms_norm_int8(x, None, None, eps=EPS)
+        _check_rows(type(r8)(r8.q[ends], r8.scale[ends]), _norm64(x[ends], None, None)[1])
+        dx, _ = ops.rms_norm_bwd(y, None, x, torch.ones(rows, device="cuda"), None, weight_grad=False)
+        xs, ys = x[ends].double(), y[ends].double()
+        c = (ys * xs).mean(-1, keepdim=True)
+        cabs = (ys * xs).abs().mean(-1, keepdim=True)
+        _near(dx[ends], ys - xs * c, BF16, ys.abs() + xs.abs() * cabs, "dx")
+        del x, y, h, r8, dx
+
+
 def test_runs_on_the_current_stream():
     """Inputs written on a side stream just before the call, on that stream."""
     from race_attention_b200 import add_rms_norm
