@@ -43,6 +43,7 @@ struct RowArgs {
   int K, w_bf16;
   float eps;
   int q_vec = 0;  // 8-byte stores of 8-bit rows
+  float inv_K = 0.f;
 };
 
 __device__ __forceinline__ float weight_at(const void *w, int w_bf16, long long i) {
@@ -75,16 +76,17 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t v, float *red) {
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// q = round(127 y / amax).  Rows of magnitudes near the smallest floats are first scaled by
-// 2^100 (`lift`), so that 127 / amax does not overflow.  A row of zeros gives 0 * infinity, and
+// q = round(127 y / amax).  Rows of magnitudes near the ends of fp32's range are first scaled by
+// a power of two (`lift`), so that neither 127 / amax overflows nor the approximate quotient,
+// which is 0 from denominators of 2^126 on, is wrong.  A row of zeros gives 0 * infinity, and
 // the conversion of a NaN to an integer 0.
 struct Quantiser {
   float scale, lift, inv;
   __device__ __forceinline__ explicit Quantiser(uint32_t amax_bits) {
     const float amax = __uint_as_float(amax_bits);
-    scale = amax / 127.f;
-    lift = amax < 1e-30f ? 0x1p100f : 1.f;
-    inv = 127.f / (amax * lift);
+    scale = amax * (1.f / 127.f);
+    lift = amax < 1e-30f ? 0x1p100f : amax > 1e30f ? 0x1p-100f : 1.f;
+    inv = __fdividef(127.f, amax * lift);
   }
   __device__ __forceinline__ int operator()(float lifted) const { return __float2int_rn(lifted * inv); }
 };
@@ -390,8 +392,10 @@ __device__ __forceinline__ int group_size() {
 
 // What bounds it is the rows' one trip from and to HBM; see launch_width for the widths' groups
 // and what they measured.
+// (least blocks per SM: what bounds the registers, see launch_width)
+constexpr int row_blocks(int G, int VPT) { return G == 512 ? 3 : G == 288 ? (VPT == 4 ? 4 : 5) : 1; }
 template <typename T, int MODE, int G, int VPT, int LAYOUT>
-__global__ void __launch_bounds__(row_block(G)) row_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(row_block(G), row_blocks(G, VPT)) row_kernel(const RowArgs a) {
   __shared__ float red_sum[2][32];
   __shared__ uint32_t red_max[2][32];
   constexpr int kPer = row_block(G) / G;  // rows of a block at a time
@@ -446,7 +450,7 @@ __global__ void __launch_bounds__(row_block(G)) row_kernel(const RowArgs a) {
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < VPT * 8; ++i) ss = fmaf(v[i], v[i], ss);
-      const float rstd = rsqrtf(group_sum<G>(ss, red_sum[flip]) / (float)K + a.eps);
+      const float rstd = rsqrtf(group_sum<G>(ss, red_sum[flip]) * a.inv_K + a.eps);
       if (a.rstd && tid == 0) a.rstd[row] = rstd;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
@@ -538,6 +542,7 @@ struct BwdArgs {
   float *part;  // [blocks, K] partial sums of dw
   long long rows;
   int K, w_bf16;
+  float inv_K = 0.f;
 };
 
 // Any width: a block takes rows blockIdx.x, blockIdx.x + gridDim.x, ...; its share of
@@ -623,7 +628,7 @@ __global__ void __launch_bounds__(row_block(G), G == 320 ? 2 : 512 / row_block(G
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum = fmaf(y[j] * w[8 * i + j], x[j], sum);
     }
-    const float c = group_sum<G>(sum, red[flip]) * rstd * rstd / (float)K;
+    const float c = group_sum<G>(sum, red[flip]) * rstd * rstd * a.inv_K;
     T *dx = static_cast<T *>(a.dx) + row * K;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -768,11 +773,11 @@ void launch_row_kernel(const RowArgs &a, int vectors, cudaStream_t s) {
 }
 
 // Threads per row.  A warp up to 1024 values: no barriers, all of a row's loads in flight at
-// once.  Wider rows take a block with two vectors per thread (32768 x 2048 bf16: norm 80 us with
-// 128 threads, 83 with 64, 124 with a warp; 8-bit norm 70, 83, 132), four past 4096 values (8192:
-// norm 159 us with 256 threads, 171 with 512, 198 with 1024) except in the 8-bit norm, whose
-// registers then leave too few blocks per SM (183 us with 256, 147 with 512).  Few rows spread
-// each over more threads, for latency.
+// once.  Wider rows take a block with two vectors per thread (32768 x 2048 bf16: norm 79 us with
+// 128 threads, 83 with 64, 124 with a warp), four past 4096 values (8192: norm 157 us with 256
+// threads, 171 with 512, 198 with 1024), and blocks of registers few enough for 40 warps per SM
+// (the 8-bit norm's two kernels: 32768 x 2048 80 us without that bound, 70 with it; 16384 x 8192
+// 169 and 136).  Few rows spread each over more threads, for latency.
 template <typename T, int MODE, int LAYOUT>
 void launch_width(const RowArgs &a, cudaStream_t s) {
   const int n = (a.K + (LAYOUT == kSkewed ? 7 : 0) + 7) / 8;  // vectors, whatever the offset
@@ -783,7 +788,7 @@ void launch_width(const RowArgs &a, cudaStream_t s) {
   if (n <= 96) return launch_row_kernel<T, MODE, 32, 3, LAYOUT>(a, n, s);
   if (n <= 128) return launch_row_kernel<T, MODE, 32, 4, LAYOUT>(a, n, s);
   if (n <= 576) return launch_row_kernel<T, MODE, 288, 2, LAYOUT>(a, n, s);
-  if (n <= 1152 && (few || MODE == kNormInt8)) return launch_row_kernel<T, MODE, 576, 2, LAYOUT>(a, n, s);
+  if (n <= 1024 && few) return launch_row_kernel<T, MODE, 512, 2, LAYOUT>(a, n, s);
   if (n <= 1152) return launch_row_kernel<T, MODE, 288, 4, LAYOUT>(a, n, s);
   if (n <= 2048) return launch_row_kernel<T, MODE, 1024, 2, LAYOUT>(a, n, s);
   if constexpr (LAYOUT == kAligned) {
@@ -797,6 +802,7 @@ int past16(const void *p, int64_t bytes = 0) { return (int)((reinterpret_cast<ui
 
 template <typename T, int MODE>
 void launch_type(RowArgs a, cudaStream_t s) {
+  a.inv_K = 1.f / (float)a.K;
   const int64_t size = sizeof(T);
   a.q_vec = (reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)a.q_stride) % 8 == 0;
   if constexpr (MODE == kSwigluInt8) {
@@ -868,7 +874,8 @@ void launch_bwd_width(const BwdArgs &a, int blocks, cudaStream_t s) {
 }
 
 template <typename T>
-void launch_bwd(const BwdArgs &a, int blocks, cudaStream_t s) {
+void launch_bwd(BwdArgs a, int blocks, cudaStream_t s) {
+  a.inv_K = 1.f / (float)a.K;
   const int base = past16(a.dy);
   const bool alike = past16(a.h) == base && past16(a.dx) == base && (!a.dh || past16(a.dh) == base);
   if (alike && base == 0 && a.K % 8 == 0)
