@@ -392,10 +392,14 @@ __device__ __forceinline__ int group_size() {
 
 // What bounds it is the rows' one trip from and to HBM; see launch_width for the widths' groups
 // and what they measured.
-// (least blocks per SM: what bounds the registers, see launch_width)
-constexpr int row_blocks(int G, int VPT) { return G == 512 ? 3 : G == 288 ? (VPT == 4 ? 4 : 5) : 1; }
+// Least blocks per SM: what bounds the registers, see launch_width.  Only where that takes no
+// spills (fp32 vectors and skewed rows' weights fill them).
+template <typename T, int G, int VPT, int LAYOUT>
+constexpr int row_blocks() {
+  return sizeof(T) == 4 || LAYOUT != kAligned ? 1 : G == 512 ? 3 : G == 288 ? (VPT == 4 ? 4 : 5) : 1;
+}
 template <typename T, int MODE, int G, int VPT, int LAYOUT>
-__global__ void __launch_bounds__(row_block(G), row_blocks(G, VPT)) row_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(row_block(G), row_blocks<T, G, VPT, LAYOUT>()) row_kernel(const RowArgs a) {
   __shared__ float red_sum[2][32];
   __shared__ uint32_t red_max[2][32];
   constexpr int kPer = row_block(G) / G;  // rows of a block at a time
