@@ -396,7 +396,7 @@ __device__ __forceinline__ int group_size() {
 // spills (fp32 vectors and skewed rows' weights fill them).
 template <typename T, int G, int VPT, int LAYOUT>
 constexpr int row_blocks() {
-  return sizeof(T) == 4 || LAYOUT != kAligned ? 1 : G == 512 ? 3 : G == 288 ? (VPT == 4 ? 4 : 5) : 1;
+  return sizeof(T) == 4 || LAYOUT != kAligned ? 0 : G == 512 ? 3 : G == 288 ? (VPT == 4 ? 4 : 5) : 0;
 }
 template <typename T, int MODE, int G, int VPT, int LAYOUT>
 __global__ void __launch_bounds__(row_block(G), row_blocks<T, G, VPT, LAYOUT>()) row_kernel(const RowArgs a) {
@@ -792,6 +792,7 @@ void launch_width(const RowArgs &a, cudaStream_t s) {
   if (n <= 96) return launch_row_kernel<T, MODE, 32, 3, LAYOUT>(a, n, s);
   if (n <= 128) return launch_row_kernel<T, MODE, 32, 4, LAYOUT>(a, n, s);
   if (n <= 576) return launch_row_kernel<T, MODE, 288, 2, LAYOUT>(a, n, s);
+  if (n <= 1152 && LAYOUT != kAligned) return launch_row_kernel<T, MODE, 576, 2, LAYOUT>(a, n, s);
   if (n <= 1024 && few) return launch_row_kernel<T, MODE, 512, 2, LAYOUT>(a, n, s);
   if (n <= 1152) return launch_row_kernel<T, MODE, 288, 4, LAYOUT>(a, n, s);
   if (n <= 2048) return launch_row_kernel<T, MODE, 1024, 2, LAYOUT>(a, n, s);
