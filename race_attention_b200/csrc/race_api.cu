@@ -767,8 +767,9 @@ uint32_t current_wait_limit() { return wait_limit(); }
 bool status_check_on() { return g_status_check.load(std::memory_order_relaxed) != 0; }
 bool withhold_first_load() { return g_withhold_first_load.load(std::memory_order_relaxed) != 0; }
 
+bool bind_context() { return fasthost::bind_current_context(); }
+
 bool make_byte_rows_map(void *map, const void *base, int64_t rows, int64_t cols, int64_t row_stride, int box_rows) {
-  if (!fasthost::bind_current_context()) return false;
   fasthost::EncodeTiledFn enc = fasthost::encoder();
   if (!enc) return false;
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
