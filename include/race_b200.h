@@ -431,8 +431,8 @@ int race_int8_linear(const int8_t *xq, int64_t x_stride, const float *x_scale, c
  *   logp = z[token] - log sum exp z;  entropy = -sum p log p (nats)
  *   top_ids / top_logp [rows, n_top]: the n_top <= min(32, V) largest entries in the
  *   order (value descending, index ascending) and their log probabilities.
- * lse [rows, 2] (8-byte aligned) is what the backward takes: the largest logit, and
- * log2 of the sum of exp(z) relative to its own.  Entries of -infinity have probability 0; a row
+ * lse [rows, 2] (8-byte aligned; may be NULL) is what the backward takes: the largest
+ * logit, and log2 of the sum of exp(z) relative to its own.  Entries of -infinity have probability 0; a row
  * of them alone has logp -infinity and entropy 0.  A NaN or +infinity in a row makes its logp and entropy NaN
  * (a NaN ranks as -infinity among the alternatives).  A row whose token is ignore_index
  * has logp and entropy 0, ids -1 and top_logp -infinity; any other token outside

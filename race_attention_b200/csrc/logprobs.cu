@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
     if (rank == 0 && tid == 0) {
       a.logp[row] = 0.f;
       a.entropy[row] = 0.f;
-      a.lse[row] = make_float2(0.f, 0.f);
+      if (a.lse) a.lse[row] = make_float2(0.f, 0.f);
     }
     if (rank == 0 && tid < a.n_top) {
       a.top_ids[row * a.n_top + tid] = -1;
@@ -349,15 +349,13 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
         }
       }
     };
-    if (kNT == 32 && g1 - g0 <= 8 * kNT) {  // each lane its own few granules
-      if (mine && mine >= t)
-        for (int j = g0 + tid; j < g1; j += kNT) offer(j);
-    } else {  // a warp at a time for each thread that has some
-      if (mine && mine >= t) owner[atomicAdd(&n_owner, 1)] = tid;
-      __syncthreads();
-      const int owners = n_owner;
-      for (int w = warp; w < owners; w += kWarps)
-        for (int j = g0 + owner[w] + lane * kNT; j < g1; j += 32 * kNT) offer(j);
+    if (mine && mine >= t) owner[atomicAdd(&n_owner, 1)] = tid;
+    __syncthreads();
+    // the owners' granules, dealt out to all threads
+    const int each = (g1 - g0 + kNT - 1) / kNT, items = n_owner * each;
+    for (int i = tid; i < items; i += kNT) {
+      const int j = g0 + owner[i / each] + i % each * kNT;
+      if (j < g1) offer(j);
     }
     __syncthreads();
     const int n = n_cand;
@@ -436,7 +434,7 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
   const float lm = all.m == -INFINITY ? 0.f : all.m, log_s = empty ? -INFINITY : log2f(all.s);
   auto log_p = [&](float l) { return empty ? -INFINITY : (l - lm) * a.inv_temp - log_s * kLn2; };
   if (tid == 0) {
-    a.lse[row] = make_float2(lm, log_s);
+    if (a.lse) a.lse[row] = make_float2(lm, log_s);
     a.entropy[row] = empty ? 0.f : (log_s - all.u / all.s) * kLn2;
     a.logp[row] = token < 0 || token >= a.V ? NAN : log_p(to_f<T>(view.row[token]));
   }
@@ -683,7 +681,7 @@ extern "C" {
 int race_token_logprobs_fwd(const void *logits, int64_t stride, int dtype, const int64_t *tokens, int64_t ignore_index,
                             float temperature, int n_top, float *logp, float *entropy, float *lse, int64_t *top_ids,
                             float *top_logp, int64_t rows, int64_t V, void *stream) {
-  if (!logits || !tokens || !logp || !entropy || !lse || (n_top > 0 && (!top_ids || !top_logp)))
+  if (!logits || !tokens || !logp || !entropy || (n_top > 0 && (!top_ids || !top_logp)))
     return err(RACE_ERR_ARG, "race_token_logprobs_fwd: null pointer");
   if (reinterpret_cast<uintptr_t>(lse) & 7) return err(RACE_ERR_ALIGN, "race_token_logprobs_fwd: lse must be 8-byte aligned");
   if (const int rc = check_shape(rows, V, stride, dtype, temperature)) return rc;

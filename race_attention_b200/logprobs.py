@@ -54,5 +54,6 @@ def token_logprobs(logits, tokens, temperature=1.0, n_top=0, ignore_index=-100) 
     and no gradient; the mean of -logp over the other rows is the cross entropy."""
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*TokenLogprobsFn.apply(logits, tokens, temperature, n_top, ignore_index))
-    logp, entropy, _, top_ids, top_logp = ops.token_logprobs_fwd(logits, tokens, temperature, n_top, ignore_index)
+    logp, entropy, _, top_ids, top_logp = ops.token_logprobs_fwd(logits, tokens, temperature, n_top, ignore_index,
+                                                                 keep_lse=False)
     return TokenLogprobs(logp, entropy, top_ids, top_logp)

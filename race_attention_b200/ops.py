@@ -27,15 +27,16 @@ def _stream(dev):
 
 
 def _check_cuda(*ts):
-    dev = None
+    dev, index = None, -1
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device()  # -1: not on a GPU
+        if i < 0:
             raise RuntimeError("CUDA only")
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
+            dev, index = t.device, i
+        elif i != index:
             raise RuntimeError("all tensors must be on the same CUDA device")
     return dev
 
@@ -515,15 +516,19 @@ def gqa_decode_attention(q, k_new, v_new, k_cache, v_cache, length, workspace, n
 # probabilities.  Some of them run for a few microseconds on a decode step, so their checks
 # are single passes over attributes and they launch without entering a device context where
 # the tensors' device is current.
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _launch(dev, name, *args):
     """Call C entry point `name` with args and the current stream of `dev`."""
     fn = getattr(_lib.load(), name)
     index = dev.index
-    if index == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index == _current_device():
+        rc = fn(*args, _current_stream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(*args, _current_stream(index))
     if rc:
         _lib.check(rc, name)
 
@@ -531,12 +536,13 @@ def _launch(dev, name, *args):
 def _rows(x, name):
     """x [..., K] as (rows with unit stride inside a row, row stride, rows, K): a view where
     the rows are evenly spaced, else a copy."""
-    if x.dim() < 1 or x.shape[-1] < 1:
+    shape = x.shape
+    if not shape or not shape[-1]:
         raise RuntimeError(f"{name} must have rows of at least one value")
-    K = x.shape[-1]
+    K = shape[-1]
     if x.is_contiguous():
         return x, K, x.numel() // K, K
-    if x.dim() != 2:
+    if len(shape) != 2:
         x = x.reshape(-1, K)
     rows, stride = x.shape[0], x.stride(0)
     if x.stride(1) != 1 or (stride < K and rows > 1):  # strided or overlapping (expanded) rows
@@ -569,7 +575,7 @@ def _ptr_of(t):
 
 
 def _dense_like(x):
-    return torch.empty_like(x, memory_format=torch.contiguous_format)
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def rms_norm_fwd(x, residual=None, weight=None, eps=1e-5, return_rstd=False):
@@ -623,9 +629,12 @@ def rms_norm_bwd_unchecked(dy, dh, h, rstd, weight, weight_grad):
 def _int8_out(x, K):
     """8-bit rows [..., K] (for x [..., *]) that start at multiples of 16 bytes, as the 8-bit
     product's tile loads need, their row stride, and their scales [...]."""
-    lead = x.shape[:-1]
+    shape = x.shape
+    lead = shape[:-1]
     scale = x.new_empty(lead, dtype=torch.float32)
     if K % 16 == 0:
+        if K == shape[-1] and x.is_contiguous():
+            return torch.empty_like(x, dtype=torch.int8), K, scale
         return x.new_empty(lead + (K,), dtype=torch.int8), K, scale
     stride = -(-K // 16) * 16
     return x.new_empty(lead + (stride,), dtype=torch.int8)[..., :K], stride, scale
@@ -676,23 +685,20 @@ def dequant_int8(q, scale, dtype=torch.bfloat16):
     """q * scale, rounded to dtype."""
     dev = _check_cuda(q, scale)
     qr, qs, rows, K, scale = _int8_rows(q, scale, "q")
-    out = q.new_empty(q.shape, dtype=dtype)
+    out = torch.empty_like(q, dtype=dtype, memory_format=torch.contiguous_format)
     if rows:
         _launch(dev, "race_dequant_int8", qr.data_ptr(), qs, scale.data_ptr(), out.data_ptr(), _dtype_code(out), rows, K)
     return out
 
 
-def _aligned_rows(q, stride):
-    """8-bit rows whose starts are multiples of 16 bytes: q, or a padded copy of it."""
-    K = q.shape[-1]
-    if q.data_ptr() % 16 == 0:
-        if stride % 16 == 0:
-            return q, stride
-        if q.numel() == K:  # a single row: nothing lies a stride further on
-            return q, -(-K // 16) * 16
+def _aligned_rows(q, rows, K):
+    """8-bit rows whose starts are multiples of 16 bytes, and their stride: a padded copy of q, or
+    q itself where it is a single row that starts at one."""
     stride = -(-K // 16) * 16
-    p = q.new_empty((q.numel() // K, stride))[:, :K]
-    p.copy_(q.reshape(-1, K))
+    if rows == 1 and q.data_ptr() % 16 == 0:
+        return q, stride
+    p = q.new_empty((rows, stride))[:, :K]
+    p.copy_(q.reshape(rows, K))
     return p, stride
 
 
@@ -702,18 +708,20 @@ def int8_linear(xq, x_scale, wq, w_scale, bias=None, dtype=torch.bfloat16):
     here lay them out) are read in place; others are copied first."""
     dev = _check_cuda(xq, x_scale, wq, w_scale, bias)
     xr, xs, M, K, x_scale = _int8_rows(xq, x_scale, "x")
-    if wq.dim() != 2 or wq.shape[1] != K:
+    wr, ws, N, Kw, w_scale = _int8_rows(wq, w_scale, "w")
+    if Kw != K or wq.dim() != 2:
         raise RuntimeError(f"w must be int8 [N, {K}]")
-    wr, ws, N, _, w_scale = _int8_rows(wq, w_scale, "w")
     if bias is not None and (bias.shape != (N,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
         raise RuntimeError(f"bias must be a contiguous float32 [{N}] tensor")
     code = _dtype_code_of(dtype)
-    y = xq.new_empty(xq.shape[:-1] + (N,), dtype=dtype)
+    y = xq.new_empty((M, N) if xq.dim() == 2 else xq.shape[:-1] + (N,), dtype=dtype)
     if M and N:
-        xr, xs = _aligned_rows(xr, xs)
-        wr, ws = _aligned_rows(wr, ws)
+        if xs % 16 or xr.data_ptr() % 16:
+            xr, xs = _aligned_rows(xr, M, K)
+        if ws % 16 or wr.data_ptr() % 16:
+            wr, ws = _aligned_rows(wr, N, K)
         _launch(dev, "race_int8_linear", xr.data_ptr(), xs, x_scale.data_ptr(), wr.data_ptr(), ws, w_scale.data_ptr(),
-                _ptr_of(bias), y.data_ptr(), code, M, N, K)
+                None if bias is None else bias.data_ptr(), y.data_ptr(), code, M, N, K)
     return y
 
 
@@ -724,20 +732,20 @@ def _logit_rows(logits, tokens):
     return dev, _dtype_code(logits), *_rows(logits, "logits"), tokens.contiguous()
 
 
-def token_logprobs_fwd(logits, tokens, temperature=1.0, n_top=0, ignore_index=-100):
+def token_logprobs_fwd(logits, tokens, temperature=1.0, n_top=0, ignore_index=-100, keep_lse=True):
     """(logp, entropy, lse, top_ids, top_logp) of logits [..., V] at tokens [...]; the last two are
-    [..., n_top], lse [..., 2] is for the backward.  See race_token_logprobs_fwd in include/race_b200.h for masked and ignored rows."""
+    [..., n_top], lse [..., 2] is for the backward (None unless keep_lse).  See race_token_logprobs_fwd in include/race_b200.h for masked and ignored rows."""
     dev, code, lr, ls, rows, V, tokens = _logit_rows(logits, tokens)
     n_top = int(n_top)
     shape = tokens.shape
     logp = torch.empty_like(tokens, dtype=torch.float32)
     entropy = torch.empty_like(logp)
-    lse = logp.new_empty(shape + (2,))
+    lse = logp.new_empty(shape + (2,)) if keep_lse else None
     top_logp = logp.new_empty(shape + (max(n_top, 0),))
     top_ids = torch.empty_like(top_logp, dtype=torch.int64)
     if rows:
         _launch(dev, "race_token_logprobs_fwd", lr.data_ptr(), ls, code, tokens.data_ptr(), int(ignore_index),
-                float(temperature), n_top, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top_ids.data_ptr(),
+                float(temperature), n_top, logp.data_ptr(), entropy.data_ptr(), _ptr_of(lse), top_ids.data_ptr(),
                 top_logp.data_ptr(), rows, V)
     return logp, entropy, lse, top_ids, top_logp
 

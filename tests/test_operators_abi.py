@@ -63,7 +63,7 @@ def logp_bwd(l=P, st=100, dt=F32, t=P, temp=1.0, lse=P, e=P, d=P, rows=4, V=100)
     (swiglu, [dict(x=None), dict(q=None), dict(s=None)]),
     (dequant, [dict(q=None), dict(s=None), dict(o=None)]),
     (linear, [dict(x=None), dict(s=None), dict(w=None), dict(t=None), dict(y=None)]),
-    (logp_fwd, [dict(l=None), dict(t=None), dict(lp=None), dict(e=None), dict(lse=None), dict(ids=None), dict(top=None)]),
+    (logp_fwd, [dict(l=None), dict(t=None), dict(lp=None), dict(e=None), dict(ids=None), dict(top=None)]),
     (logp_bwd, [dict(l=None), dict(t=None), dict(lse=None), dict(e=None), dict(d=None)]),
 ])
 def test_null_pointers_and_dtypes(call, bad):
