@@ -579,12 +579,13 @@ __global__ void __launch_bounds__(kNT) bwd_loop_kernel(BwdArgs a) {
 }
 
 // A group of G threads walks rows; a thread keeps its columns' weights and sums of dw in
-// registers over all of them, and where the group is a block (whose barrier every row pays) it
-// has the next row's values on their way while it works on this one's.
+// registers over all of them, and has the next row's values on their way while it works on this
+// one's where they are few or the group is a block (whose barrier every row pays): 200000 x 256
+// bf16 124 us without, 105 with.
 template <typename T, int G, int VPT, int LAYOUT>
 __global__ void __launch_bounds__(row_block(G), G == 320 ? 2 : 512 / row_block(G)) bwd_kernel(const BwdArgs a) {
   constexpr int kPer = row_block(G) / G, N = VPT * 8;
-  constexpr bool kAhead = G > 32;
+  constexpr bool kAhead = G > 32 || VPT * sizeof(T) <= 4;  // (the registers of wider warps' rows would spill)
   __shared__ float red[2][32];
   extern __shared__ float warp_dw[];  // [groups of the block][K], where a block has several
   const int size = group_size<G>(), tid = G == 32 ? threadIdx.x % 32 : threadIdx.x, K = a.K;
@@ -839,10 +840,10 @@ int launch_rows(const char *what, const RowArgs &a, int dtype, cudaStream_t s) {
 }
 
 // Blocks of the backward, each with one row of partial sums of dw to be added: four per SM of
-// a B200, eight where they are of 64 threads; with few rows a row each, then four (in a warp
-// of its own each up to 768 values).  A multiple of 8 (see kSkewed).
+// a B200, two where they hold eight rows at a time (up to 768 values), eight where they are of 64
+// threads; with few rows a row each, then four.  A multiple of 8 (see kSkewed).
 int bwd_blocks(int64_t rows, int64_t K) {
-  const int64_t n = rows <= 148 ? rows : rows <= 592 ? 148 : (rows + 3) / 4, most = K > 768 && K <= 1024 ? 1184 : 592;
+  const int64_t n = rows <= 148 ? rows : rows <= 592 ? 148 : (rows + 3) / 4, most = K <= 768 ? 296 : K <= 1024 ? 1184 : 592;
   return (int)(n < most ? (n + 7) / 8 * 8 : most);
 }
 
