@@ -46,7 +46,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
     cuda_home = os.path.dirname(os.path.dirname(_nvcc()))
     cmd = [
         _nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr",
-        "-Xcompiler", "-fPIC,-O3", "-shared", "-cudart", "shared",
+        "-Xcompiler", "-fPIC,-O3", "-shared", "-cudart", "shared", "--threads", "0",
         "-I", INCLUDE, "-I", CSRC,
         "-Xlinker", f"-rpath,{os.path.join(cuda_home, 'lib64')}",
         "-o", LIB + ".tmp", *sorted(glob.glob(os.path.join(CSRC, "*.cu"))),
