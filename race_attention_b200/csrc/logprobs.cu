@@ -435,7 +435,8 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
   auto log_p = [&](float l) { return empty ? -INFINITY : (l - lm) * a.inv_temp - log_s * kLn2; };
   if (tid == 0) {
     if (a.lse) a.lse[row] = make_float2(lm, log_s);
-    a.entropy[row] = empty ? 0.f : (log_s - all.u / all.s) * kLn2;
+    const float entropy = empty ? 0.f : (log_s - all.u / all.s) * kLn2;
+    a.entropy[row] = entropy < 0.f ? 0.f : entropy;  // (rounding; a NaN stays)
     a.logp[row] = token < 0 || token >= a.V ? NAN : log_p(to_f<T>(view.row[token]));
   }
   const int n = C * a.n_top;

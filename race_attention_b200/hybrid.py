@@ -30,7 +30,7 @@ import torch.nn.functional as F
 from . import ops
 from .decode import RaceDecodeState, prefill_with_state
 from .int8 import Int8Linear, add_rms_norm_int8, swiglu_int8
-from .logprobs import token_logprobs
+from .logprobs import TokenLogprobs, token_logprobs
 from .race_common import build_planes_protos
 
 
@@ -253,10 +253,10 @@ class HybridLlama(nn.Module):
         """TokenLogprobs of idx [B, T]: token t's log probability given those before it, [B, T - 1]
         (no caches kept); logits exist for `positions` positions at a time."""
         logits = self._forward_only(idx)
-        parts = [token_logprobs(logits(slice(t, min(t + positions, idx.shape[1] - 1))),
-                                idx[:, t + 1:min(t + positions, idx.shape[1] - 1) + 1], temperature, n_top)
-                 for t in range(0, idx.shape[1] - 1, positions)]
-        return type(parts[0])(*(torch.cat(c, 1) for c in zip(*parts)))
+        n = idx.shape[1] - 1
+        parts = [token_logprobs(logits(slice(t, min(t + positions, n))), idx[:, t + 1:min(t + positions, n) + 1],
+                                temperature, n_top) for t in range(0, max(n, 1), positions)]
+        return TokenLogprobs(*(torch.cat(c, 1) for c in zip(*parts)))
 
     def _step_logits(self, tok):
         """One decode step on the device: every position-dependent value comes from self.pos,

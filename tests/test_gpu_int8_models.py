@@ -91,6 +91,8 @@ def test_answers_with_log_probabilities(int8):
     last = full.logits_full(idx[:, :-1]).double().log_softmax(-1).gather(-1, idx[:, -1:])[:, 0]
     assert bool(((s.logp[:, -1].double() - last).abs() < 0.05 * last.abs()).all())
     assert full.pos is None  # scoring keeps no decode state
+    one = full.score(idx[:, :1], n_top=2)  # nothing to score in a single token
+    assert one.logp.shape == (2, 0) and one.top_ids.shape == (2, 0, 2)
 
 
 def _gpt(fused):

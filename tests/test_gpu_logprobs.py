@@ -187,6 +187,16 @@ def test_gradient_against_differences():
     assert abs((f(step) - f(-step)) / (2 * step) - slope) < bound
 
 
+def test_entropies_are_not_negative():
+    """Peaked rows, whose entropy is below the rounding of its terms."""
+    from race_attention_b200 import token_logprobs
+    g = _gen(26)
+    logits = torch.randn(4000, 97, generator=g, device="cuda")
+    logits[:, 3] += torch.linspace(5, 60, 4000, device="cuda")
+    got = token_logprobs(logits, torch.full((4000,), 3, device="cuda"))
+    assert bool((got.entropy >= 0).all()) and bool((got.logp <= 0).all())
+
+
 def test_cross_entropy_is_the_mean_of_the_rest():
     from race_attention_b200 import token_logprobs
     g = _gen(22)
