@@ -23,16 +23,6 @@ bool withhold_first_load();     // race_test_withhold_first_load()
 bool bind_context();
 bool make_byte_rows_map(void *map, const void *base, int64_t rows, int64_t cols, int64_t row_stride, int box_rows);
 
-uint32_t current_wait_limit();  // race_set_wait_limit()'s value for the next launch
-bool status_check_on();         // race_set_status_check()
-bool withhold_first_load();     // race_test_withhold_first_load()
-// Tensor map of rows x cols bytes (row stride a multiple of 16 bytes) in boxes of
-// box_rows x 128 bytes, 128-byte swizzle; out-of-range bytes read as 0.  False if the
-// driver refuses it.  `map` points at a CUtensorMap.  A thread that has only queried the
-// runtime calls bind_context() first.
-bool bind_context();
-bool make_byte_rows_map(void *map, const void *base, int64_t rows, int64_t cols, int64_t row_stride, int box_rows);
-
 // Fails with `code`: formats the detail of race_last_error().
 inline int err(int code, const char *fmt, long long a = 0, long long b = 0) {
   char buf[256];

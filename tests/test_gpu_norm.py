@@ -202,6 +202,21 @@ def test_int8_rows(rows, K, dtype):
     _check_rows(swiglu_int8(gu), gate * torch.sigmoid(gate) * up)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,K,pad", [(1189, 2056, 0), (1187, 2048, 8), (1250, 4096, 16), (1190, 2048, 3), (1186, 2041, 7),
+                                        (80003, 24, 0), (76802, 32, 8), (303107, 8, 8)])
+def test_dequant_of_many_rows(rows, K, pad, dtype):
+    # groups of rows that the last thread has only some of; row strides that are and are not whole words
+    from race_attention_b200 import Int8Rows
+    g = _gen(rows + K)
+    q = torch.randint(-127, 128, (rows, K + pad), generator=g, device="cuda", dtype=torch.int8)[:, :K]
+    scale = torch.rand(rows, generator=g, device="cuda") + 0.01
+    got = Int8Rows(q, scale).dequant(dtype)
+    assert got.shape == (rows, K) and got.dtype == dtype
+    # one product in 32 bits, rounded once more for bf16
+    assert torch.equal(got, (q.double() * scale.double()[:, None]).to(F32).to(dtype))
+
+
 def test_int8_rows_of_zeros_tiny_and_huge_values():
     from race_attention_b200 import quant_int8
     x = torch.zeros(6, 100, device="cuda")
