@@ -398,8 +398,9 @@ int race_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float
                       int weight_dtype, void *dx, void *dw, int64_t rows, int64_t K, void *workspace,
                       size_t workspace_bytes, void *stream);
 
-/* 8-bit rows: q[r, k] = round_to_nearest_even(v[r, k] / scale[r]), scale[r] =
- * max_k |v[r, k]| / 127 (fp32).  A row of zeros has scale 0 and q = 0; a row holding a
+/* 8-bit rows: scale[r] = max_k |v[r, k]| times the fp32 number nearest to 1/127, rounded to
+ * fp32, and q[r, k] = round_to_nearest_even(v[r, k] / scale[r]), the quotient rounded to fp32
+ * first (a division), within [-127, 127].  A row of zeros has scale 0 and q = 0; a row holding a
  * NaN has scale NaN, one holding an infinity scale infinity (so products of it are not
  * finite).  q_stride (bytes) >= K; race_int8_linear wants it a multiple of 16.
  *   race_quant_int8:     v = x

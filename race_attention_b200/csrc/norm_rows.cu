@@ -7,10 +7,12 @@
 //   rstd = 1 / sqrt(mean(h^2) + eps),   y = h * rstd * w
 //   backward, g = dy * w:  dx = dr = rstd * (g - h * rstd^2 * mean(g * h)) + dh,
 //                          dw = sum over rows of dy * h * rstd
-//   8-bit row of y: scale = max|y| / 127, q = round_to_even(y / scale)
+//   8-bit row of y: scale = max|y| times fp32's 1/127, q = round_to_even(y / scale), the quotient
+//                   correctly rounded
 // Sums, statistics and everything up to the last rounding are fp32.
 //
-// A row of zeros has scale 0 and q = 0.  A row that holds a NaN (or whose largest
+// A row of zeros (or of values under 2^-143, whose scale fp32 does not hold) has scale 0 and q = 0.
+// A row that holds a NaN (or whose largest
 // magnitude is infinite) has scale NaN (infinity), so whatever is computed from it
 // is not finite either; no such row touches another.
 #include "race_b200.h"
@@ -76,19 +78,59 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t v, float *red) {
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// q = round(127 y / amax).  Rows of magnitudes near the ends of fp32's range are first scaled by
-// a power of two (`lift`), so that neither 127 / amax overflows nor the approximate quotient,
-// which is 0 from denominators of 2^126 on, is wrong.  A row of zeros gives 0 * infinity, and
-// the conversion of a NaN to an integer 0.
+// four values to signed bytes (the conversion saturates)
+__device__ __forceinline__ uint32_t pack_s8(int a, int b, int c, int d) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\t"
+      "cvt.pack.sat.s8.s32.b32 t, %4, %3, 0;\n\t"
+      "cvt.pack.sat.s8.s32.b32 %0, %2, %1, t;\n\t}"
+      : "=r"(r)
+      : "r"(a), "r"(b), "r"(c), "r"(d));
+  return r;
+}
+
+// q = round_to_even(y / scale), where the quotient is rounded to fp32 as a division does: values on
+// half a step are common among bf16 rows, and there the last place decides.  Markstein's method: t =
+// y (1 / scale), then one step with the residual y - t scale, which the fused multiply-add gives
+// exactly; the reciprocal has had a step of Newton's.  On a B200 the result rounds to the same
+// integer as the division's for every significand of the scale and every y within four places of
+// half a step (all enumerated; of those 3 % are off by the reciprocal alone).  What it costs next to
+// that one product: 8-bit norm 32768 x 2048 bf16 72 us and 70.5, rows to 8 bits 37 and 36, 16384 x
+// 8192 70 and 64.
+// Rows near the ends of fp32's range are first scaled by a power of two (`lift`, which changes no
+// quotient), so that their residuals are exact too.  A scale among the subnormals may be well under
+// max|y| / 127: such a row's values are held at 127 steps.  Where the scale is 0 or not finite the
+// quotients are NaN, and the conversion of a NaN to an integer 0.
 struct Quantiser {
-  float scale, lift, inv;
+  float scale, lift, unit, inv;
   __device__ __forceinline__ explicit Quantiser(uint32_t amax_bits) {
     const float amax = __uint_as_float(amax_bits);
     scale = amax * (1.f / 127.f);
-    lift = amax < 1e-30f ? 0x1p100f : amax > 1e30f ? 0x1p-100f : 1.f;
-    inv = __fdividef(127.f, amax * lift);
+    lift = amax < 1e-25f ? 0x1p100f : amax > 1e30f ? 0x1p-100f : 1.f;
+    unit = scale * lift;
+    const float y = __fdividef(1.f, unit);
+    inv = fmaf(fmaf(-unit, y, 1.f), y, y);
   }
-  __device__ __forceinline__ int operator()(float lifted) const { return __float2int_rn(lifted * inv); }
+  __device__ __forceinline__ float lifted(float y) const {
+    const float most = 127.f * unit;
+    return fminf(fmaxf(y * lift, -most), most);
+  }
+  // quotients (of rows that are lifted: of lifted values)
+  template <bool PAIRS>
+  __device__ __forceinline__ float2 two(float a, float b) const {
+    if constexpr (PAIRS) {
+      const float2 v = make_float2(a, b), r = make_float2(inv, inv), t = __fmul2_rn(v, r);
+      return __ffma2_rn(__ffma2_rn(t, make_float2(-unit, -unit), v), r, t);
+    } else {
+      const float t = a * inv, u = b * inv;
+      return make_float2(fmaf(fmaf(-t, unit, a), inv, t), fmaf(fmaf(-u, unit, b), inv, u));
+    }
+  }
+  template <bool PAIRS>
+  __device__ __forceinline__ uint32_t four(const float *f) const {
+    const float2 a = two<PAIRS>(f[0], f[1]), b = two<PAIRS>(f[2], f[3]);
+    return pack_s8(__float2int_rn(a.x), __float2int_rn(a.y), __float2int_rn(b.x), __float2int_rn(b.y));
+  }
 };
 
 // (the approximate quotient is 0 where the denominator passes 2^126: the product is then 0 too)
@@ -307,17 +349,6 @@ __device__ __forceinline__ void weights8(const void *w, int w_bf16, int e, int K
   }
 }
 
-// four values to signed bytes (the conversion saturates)
-__device__ __forceinline__ uint32_t pack_s8(int a, int b, int c, int d) {
-  uint32_t r;
-  asm("{\n\t.reg .b32 t;\n\t"
-      "cvt.pack.sat.s8.s32.b32 t, %4, %3, 0;\n\t"
-      "cvt.pack.sat.s8.s32.b32 %0, %2, %1, t;\n\t}"
-      : "=r"(r)
-      : "r"(a), "r"(b), "r"(c), "r"(d));
-  return r;
-}
-
 // A row's bytes, 8 per vector, to q (which starts at a multiple of 8 where `vec`).  Skewed vectors
 // start `off` bytes before multiples of 8: they go through shared memory (`line`, 8 bytes per
 // vector and 8 more), where the 8 bytes from 8 j on are 8 of a vector and the next one.
@@ -475,14 +506,18 @@ __global__ void __launch_bounds__(row_block(G), row_blocks<T, G, VPT, LAYOUT>())
       if (tid == 0) a.scale[row] = qz.scale;
       if (qz.lift != 1.f) {
 #pragma unroll
-        for (int i = 0; i < VPT * 8; ++i) v[i] *= qz.lift;
+        for (int i = 0; i < VPT * 8; ++i) v[i] = qz.lifted(v[i]);
       }
       int8_t *q = a.q + row * a.q_stride;
       uint2 b[VPT];
+      // By pairs of values unless their registers cost a block per SM or spill (bf16: 8-bit norm of
+      // 16384 x 8192 139 us by single values and 155 by pairs, rows of 16384 values to 8 bits 193
+      // and 260; elsewhere 16384 x 8192 SwiGLU 104 us by pairs and 108 by single values, 262144 x
+      // 256 to 8 bits 41 and 42).
+      constexpr bool kPairs = G < 1024 && !(MODE == kNormInt8 && VPT == 4);
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        const float *f = v + 8 * i;
-        b[i] = make_uint2(pack_s8(qz(f[0]), qz(f[1]), qz(f[2]), qz(f[3])), pack_s8(qz(f[4]), qz(f[5]), qz(f[6]), qz(f[7])));
+        b[i] = make_uint2(qz.four<kPairs>(v + 8 * i), qz.four<kPairs>(v + 8 * i + 4));
       }
       store_bytes<VPT, G, LAYOUT>(q, b, line + (threadIdx.x / 32) * (G == 32 ? VPT * 32 + 1 : 0), off, tid, size, K, a.q_vec);
     }
@@ -534,7 +569,8 @@ __global__ void __launch_bounds__(kNT) row_loop_kernel(RowArgs a) {
   if (threadIdx.x == 0) a.scale[row] = qz.scale;
   int8_t *q = a.q + row * a.q_stride;
   for (int i = threadIdx.x; i < K; i += kNT) {
-    q[i] = (int8_t)qz(value(i) * qz.lift);
+    const float v = value(i);
+    q[i] = (int8_t)__float2int_rn(qz.two<false>(qz.lifted(v), 0.f).x);
     if (MODE == kNormInt8 && r) h[i] = from_f<T>(stream(i));
   }
 }

@@ -5,8 +5,9 @@ serving path of a decoder whose projections run on 8-bit integer tensor cores).
     y = int8_linear(rows, weight_rows)               # weight_rows = quant_int8(linear.weight)
     down = int8_linear(swiglu_int8(gate_up), down_rows)
 
-A row is q[k] = round(v[k] / scale), scale = max|v| / 127: symmetric, one scale per token for
-activations and one per output channel for weights.
+A row is q[k] = round(v[k] / scale), scale = max|v| times fp32's 1/127, the same numbers as a
+division in fp32 gives: symmetric, one scale per token for activations and one per output channel
+for weights.
 """
 from __future__ import annotations
 

@@ -202,6 +202,41 @@ def test_int8_rows(rows, K, dtype):
     _check_rows(swiglu_int8(gu), gate * torch.sigmoid(gate) * up)
 
 
+def _quotients(x):
+    """Scales and 8-bit values by the definition: scale = max|x| times fp32's 1/127, the quotients
+    rounded to fp32 as a division's are (from 64 bits: as many as that takes), then to whole numbers."""
+    x = x.double()
+    scale = (x.abs().amax(-1) * float(torch.tensor(1 / 127, dtype=F32))).to(F32)
+    q = (x / scale.double()[..., None]).to(F32).round().clamp(-127, 127)
+    return torch.where(scale[..., None] > 0, q, torch.zeros_like(q)).to(torch.int8), scale
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,K", [(2000, 256), (64, 2048), (3000, 768), (700, 1000), (300, 2047), (100, 8192), (1500, 4096),
+                                    (41, 8191), (20, 16384), (9, 40001)])
+def test_int8_rows_are_the_quotients(rows, K, dtype):
+    """Every value, those on half a step among them (which bf16 rows often hold): no tolerance."""
+    from race_attention_b200 import quant_int8
+    x = torch.randn(rows, K, generator=_gen(rows + 2 * K), device="cuda").to(dtype)
+    x[0] = torch.arange(K, device="cuda") % 255 - 127  # halves and whole numbers of steps alone
+    x[0, 0] = 63.5
+    for v in (x, torch.cat([x, x], 1)[:, 1:K + 1]):
+        got = quant_int8(v)
+        q, scale = _quotients(v)
+        assert torch.equal(got.scale, scale) and torch.equal(got.q, q)
+
+
+@pytest.mark.parametrize("K", [96, 331, 2048, 40001])
+def test_int8_rows_are_the_quotients_at_the_ends_of_the_range(K):
+    from race_attention_b200 import quant_int8
+    e = torch.arange(-149, 128, device="cuda", dtype=torch.float64)
+    v = torch.randint(-255, 256, (277, K), generator=_gen(K), device="cuda").double() / 128
+    x = (v * 2.0 ** e[:, None]).clamp(-3.3e38, 3.3e38).to(F32)
+    got = quant_int8(x)
+    q, scale = _quotients(x)
+    assert torch.equal(got.scale, scale) and torch.equal(got.q, q)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("rows,K,pad", [(1189, 2056, 0), (1187, 2048, 8), (1250, 4096, 16), (1190, 2048, 3), (1186, 2041, 7),
                                         (80003, 24, 0), (76802, 32, 8), (303107, 8, 8)])
