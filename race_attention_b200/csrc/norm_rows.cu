@@ -133,8 +133,16 @@ struct Quantiser {
   }
 };
 
-// (the approximate quotient is 0 where the denominator passes 2^126: the product is then 0 too)
-__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// g / (1 + e^-g) * u, by e^-|g|: a denominator in [1, 2], for which the reciprocal instruction needs
+// no care (the approximate quotient by one of 2^126 or more is 0, which is not what a large u makes of
+// gates below -87), and e^-|g| as the square of a number that stays normal where it does not.
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(g) * -0.7213475204444817f));  // -log2(e) / 2
+  e *= e;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return (g < 0.f ? g * e : g) * r * u;
+}
 
 // ---------------------------------------------------------------- rows in registers
 // A group of G threads owns a row and holds it in registers, so the row is read once however

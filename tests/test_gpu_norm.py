@@ -269,6 +269,23 @@ def test_int8_rows_of_zeros_tiny_and_huge_values():
     assert int(got.q[5, 99]) == -127
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("K", [64, 301, 2048, 20003])
+def test_swiglu_of_gates_far_below_zero(K, dtype):
+    """Gates whose e^-gate is near the end of fp32's range, times values that bring the products back:
+    e^-|gate| is below the normal numbers, but by less than 2^-2, so it keeps 21 bits."""
+    from race_attention_b200 import swiglu_int8
+    g = _gen(K)
+    gate = -87.4 - 1.2 * torch.rand(7, K, generator=g, device="cuda")
+    up = torch.randn(7, K, generator=g, device="cuda") * 1e37
+    gu = torch.cat([gate, up], 1).to(dtype)
+    gate, up = gu.double().chunk(2, -1)
+    _check_rows(swiglu_int8(gu), gate * torch.sigmoid(gate) * up)
+    ends = torch.tensor([[-200.0, -1e30, 0.0, -0.0, 30.0, 1e30, -20.0, 1.0] + [1.0] * 8], device="cuda").to(dtype)
+    gate, up = ends.double().chunk(2, -1)
+    _check_rows(swiglu_int8(ends), gate * torch.sigmoid(gate) * up)
+
+
 def test_int8_layouts():
     from race_attention_b200 import quant_int8, swiglu_int8
     g = _gen(5)
