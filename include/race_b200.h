@@ -444,7 +444,8 @@ int race_token_logprobs_fwd(const void *logits, int64_t stride, int dtype, const
 
 /* dlogits [rows, V] dense, of dtype, for the gradients g_logp and g_entropy [rows] fp32
  * (either may be NULL: zero) of logp and entropy, from the forward's lse and entropy.
- * Ignored rows, and rows of -infinity alone, get 0. */
+ * Ignored rows, and rows of -infinity alone, get 0.  A row whose token is outside the vocabulary
+ * gets NaN where its g_logp is not 0, else the entropy's gradient, which no token enters. */
 int race_token_logprobs_bwd(const void *logits, int64_t stride, int dtype, const int64_t *tokens, int64_t ignore_index,
                             float temperature, const float *lse, const float *entropy, const float *g_logp,
                             const float *g_entropy, void *dlogits, int64_t rows, int64_t V, void *stream);

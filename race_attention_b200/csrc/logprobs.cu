@@ -478,7 +478,8 @@ struct RowGrad {
     lm = lse.x, log_s = lse.y;
     zero = token == a.ignore || log_s == -INFINITY;
     const bool bad = token < 0 || token >= a.V;
-    const float ga = bad ? NAN : a.g_logp ? a.g_logp[row] : 0.f, gb = a.g_entropy ? a.g_entropy[row] : 0.f;
+    const float up = a.g_logp ? a.g_logp[row] : 0.f, gb = a.g_entropy ? a.g_entropy[row] : 0.f;
+    const float ga = bad && up != 0.f ? NAN : up;  // (a logp that is not used has gradient 0, NaN or not)
     A = -(ga + gb * a.entropy[row]) * a.inv_temp;
     B = -gb * kLn2 * a.inv_temp;
     one = ga * a.inv_temp;

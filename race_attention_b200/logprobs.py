@@ -51,7 +51,8 @@ def token_logprobs(logits, tokens, temperature=1.0, n_top=0, ignore_index=-100) 
     n_top <= min(32, V) alternatives per row in the order (logit descending, index ascending).
     logp and entropy are differentiable in logits; the alternatives are not.  Entries of
     -infinity (a mask) have probability 0; a row whose token is ignore_index gives 0, ids of -1
-    and no gradient; the mean of -logp over the other rows is the cross entropy."""
+    and no gradient; the mean of -logp over the other rows is the cross entropy.  Another token
+    outside the vocabulary makes its row's logp NaN, and the gradient too where that logp is used."""
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*TokenLogprobsFn.apply(logits, tokens, temperature, n_top, ignore_index))
     logp, entropy, _, top_ids, top_logp = ops.token_logprobs_fwd(logits, tokens, temperature, n_top, ignore_index,

@@ -248,6 +248,31 @@ def test_tokens_outside_the_vocabulary_give_nan():
     assert bool(d[:3].isnan().all()) and bool(d[3].isfinite().all())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [100, 1001, 33000])
+def test_tokens_outside_the_vocabulary_leave_other_gradients_alone(V, dtype):
+    """Rows whose log probability is not used (masked out, or the entropy alone taken) have the
+    gradients that any token gives them."""
+    from race_attention_b200 import token_logprobs
+    g = _gen(V + 27)
+    x = torch.randn(4, V, generator=g, device="cuda").to(dtype)
+    bad = torch.tensor([V, -1, 1 << 40, 5], device="cuda")
+    good = torch.tensor([1, 2, 3, 5], device="cuda")
+    w = torch.randn(4, generator=g, device="cuda")
+    got = []
+    for tokens in (bad, good):
+        for view in (x, torch.cat([x, x], 1)[:, 3:3 + V]):  # rows like the gradient's, and not
+            leaf = view.detach().requires_grad_(True)
+            r = token_logprobs(leaf, tokens)
+            kept = torch.where(bad == good, r.logp, torch.zeros_like(r.logp))
+            got.append([torch.autograd.grad(out, leaf, retain_graph=True)[0]
+                        for out in ((w * r.entropy).sum(), (kept * w).sum(), (kept * w).sum() + (w * r.entropy).sum())])
+    for a, b in zip(got[:2], got[2:]):
+        for da, db in zip(a, b):
+            assert bool(da.isfinite().all()) and torch.equal(da, db)
+        assert not bool(a[1][:3].any())
+
+
 def test_rows_past_two_gigabytes():
     """Offsets past 2^31 elements and 2^32 bytes: the last rows of a long batch."""
     from race_attention_b200 import token_logprobs
