@@ -372,8 +372,9 @@ __global__ void __launch_bounds__(kNT) logprobs_fwd_kernel(const FwdArgs a, cons
         if (above < a.n_top) out[above] = k;
       }
     } else {
-      // more entries reach the bound than fit (a thread's run of large ones): one pass of the
-      // share for each alternative
+      // more entries reach the bound than fit (a few threads that hold most of the large ones, or
+      // chance: about 1 % of rows of 4000 random bf16 values with 32 alternatives): one pass of
+      // the share for each alternative
       unsigned long long last = ~0ull;
       for (int i = 0; i < a.n_top; ++i) {
         unsigned long long k = 0;

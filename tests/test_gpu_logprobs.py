@@ -86,6 +86,55 @@ def test_ties_go_to_the_lowest_index(V):
         _near(got.top_logp, top, 2e-5, "top_logp")
 
 
+@pytest.mark.parametrize("V,dtype", [(4000, BF16), (2000, F32), (3993, BF16), (2047, F32)])
+def test_alternatives_of_many_random_rows(V, dtype):
+    """About one such row in a hundred has more entries at or above the bound than are ranked at once."""
+    from race_attention_b200 import token_logprobs
+    g = _gen(V + 3)
+    logits = torch.randn(4000, V, generator=g, device="cuda").to(dtype)
+    tokens = torch.zeros(4000, dtype=torch.int64, device="cuda")
+    _, _, ids, top, *_ = _reference(logits, tokens, 1.0, 32)
+    got = token_logprobs(logits, tokens, n_top=32)
+    assert torch.equal(got.top_ids, ids)
+    _near(got.top_logp, top, 2e-5, "top_logp")
+
+
+# rows, vocabulary of bf16 and fp32 rows, threads per block, blocks per row, entries ranked at once
+@pytest.mark.parametrize("rows,Vs,threads,blocks,places", [
+    (40, (4000, 2000), 32, 1, 256), (41, (2999, 2047), 32, 1, 256), (700, (10000, 8000), 128, 1, 1024),
+    (33, (9999, 7999), 128, 1, 1024), (700, (40000, 20000), 256, 1, 1024), (601, (33001, 16501), 256, 1, 1024),
+    (200, (65536, 32768), 256, 2, 1024), (3, (131072, 131072), 256, 8, 1024), (2, (200003, 160003), 256, 8, 1024)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_alternatives_that_lie_with_few_threads(rows, Vs, threads, blocks, places, dtype):
+    """The large entries of each block's share are those of n_top - 1 threads (all of them: far more than
+    are ranked at once), so the n_top-th thread's maximum, which bounds the alternatives, is low."""
+    from race_attention_b200 import token_logprobs
+    V, per = (Vs[1], 4) if dtype == F32 else (Vs[0], 8)
+    g = _gen(rows + V)
+    off = (torch.arange(rows, device="cuda") * V % per)[:, None]
+    granules = (V + off + per - 1) // per
+    granule = (torch.arange(V, device="cuda") + off) // per
+    first = torch.zeros_like(granule)  # of the block's share that a granule is in
+    for b in range(1, blocks):
+        at = granules * b // blocks
+        first = torch.where(granule >= at, at, first)
+    thread = (granule - first) % threads
+    for n in (32, 20):
+        step = max(1, threads // 32)
+        high = (thread % step == 0) & (thread // step < n - 1)
+        for b in range(blocks):
+            share = (granule >= granules * b // blocks) & (granule < granules * (b + 1) // blocks)
+            assert int((high & share).sum(1).min()) > places
+        x = torch.randn(rows, V, generator=g, device="cuda")
+        logits = torch.where(high, 10 + x.abs() / 8, x.clamp(-3, 3)).to(dtype)
+        tokens = torch.randint(0, V, (rows,), generator=g, device="cuda")
+        _, _, ids, top, *_ = _reference(logits, tokens, 1.0, n)
+        for _ in range(2):
+            got = token_logprobs(logits, tokens, n_top=n)
+            assert torch.equal(got.top_ids, ids)
+            _near(got.top_logp, top, 2e-5, "top_logp")
+
+
 @pytest.mark.parametrize("V", [5, 700, 50257])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_masks_and_rows_without_an_entry(V, dtype):
