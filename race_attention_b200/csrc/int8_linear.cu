@@ -110,6 +110,11 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void st_cluster_i(uint32_t addr, int v) {
   asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
+__device__ __forceinline__ int ld_cluster_i(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -223,9 +228,10 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__
         if (!tc::mbar_wait(&empty[st], parity, abort)) break;
         load_next();
       }
-      if (*abort)  // no copy may land after the block has gone
-        for (int k = issued > C::kStages ? issued - C::kStages : 0; k < issued; ++k)
-          tc::mbar_wait_drain(&full[k % C::kStages], (k / C::kStages) & 1);
+      // No copy may land after the block has gone, whether or not this thread learns that another
+      // one has given up (waiting for them costs nothing: the products wait for the same).
+      for (int k = issued > C::kStages ? issued - C::kStages : 0; k < issued; ++k)
+        tc::mbar_wait_drain(&full[k % C::kStages], (k / C::kStages) & 1);
     }
     __syncwarp();
     if (S > 1) cluster_wait();
@@ -245,8 +251,9 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__
         mma_stage<1>(tmem, sw, sw + kTileBytes, id, k == 0);
         tc::mma_commit(&empty[now]);
       }
+      if (*abort) __threadfence_block();  // (who sees `done` sees that it was given up)
       tc::mma_commit(&done);
-      if (*abort) tc::mbar_wait_drain(&done, 0);
+      tc::mbar_wait_drain(&done, 0);  // no product may be under way when the block goes, either
     }
     __syncwarp();
     if (S > 1) cluster_wait();
@@ -335,6 +342,11 @@ constexpr int kPairStageBytes = 2 * kTileBytes;
 constexpr int kPairN = 256;               // channels per tile and accumulator columns
 constexpr int kOutWarps = 8;              // epilogue warps: two per TMEM lane quarter, half of the columns each
 constexpr int kPairThreads = 64 + 32 * kOutWarps;
+// One arrival on this CTA's barrier once the pair's MMAs issued so far are done.
+__device__ __forceinline__ void commit_leader(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
+}
+
 // everything the pair kernel keeps in shared memory (227 KB per CTA allow one more kilobyte)
 struct PairSmem {
   unsigned char ring[kPairStages][kPairStageBytes];
@@ -342,7 +354,9 @@ struct PairSmem {
   float scale[kPairN], bias[kPairN];       // of the tile's channels
   uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2], drained;
   uint32_t tmem_slot;
-  int ctl[2];  // {abort flag, poll limit}
+  int ctl[2];   // {abort flag, poll limit}
+  int filled;   // stages this CTA has asked for
+  int gave_up;  // a wait of either CTA has
 };
 constexpr int kGroupM = 8;                // token tiles that share their weight tiles in L2
 
@@ -374,6 +388,7 @@ pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUte
     tc::prefetch_tmap(&mw);
     ctl[0] = (tc::smem_u32(ring) & 1023) != 0;  // the swizzled tiles start at multiples of 1024
     ctl[1] = (int)a.wait_limit;
+    sm.filled = sm.gave_up = 0;
     for (int i = 0; i < kPairStages; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
@@ -393,7 +408,7 @@ pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUte
 
   if (warp == 0) {
     if (lane == 0 && !a.withhold) {
-      int st = 0, filled = 0;     // the next stage, and how many are filled or were
+      int st = 0, filled = 0;     // the next stage, and how many were asked for
       uint32_t parity = 1;        // of the wait for a free stage: a fresh barrier's last phase counts as done
       bool go = true, ready = true;
       const uint32_t leader_full = map_rank(tc::smem_u32(&full[0]), 0);
@@ -415,14 +430,10 @@ pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUte
           if (rank == 0) tc::mbar_arrive_expect_tx(&full[now], 2 * kPairStageBytes);
           tma_load_pair(sa, &mx, bar, k * kBK, m);
           tma_load_pair(sa + kTileBytes, &mw, bar, k * kBK, n);
-          filled = min(filled + 1, kPairStages);
+          ++filled;
         }
       }
-      if (*abort && rank == 0)  // both CTAs' copies must have landed before either leaves
-        for (; filled > 0; --filled) {  // newest first
-          if (st-- == 0) st = kPairStages - 1, parity ^= 1;
-          tc::mbar_wait_drain(&full[st], parity ^ 1);
-        }
+      sm.filled = filled;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -453,10 +464,8 @@ pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUte
         if (go) commit_pair(&acc_full[buf]);
         if (++buf == 2) buf = 0, acc_parity ^= 1;
       }
-      if (*abort) {
-        commit_pair(&sm.drained);
-        tc::mbar_wait_drain(&sm.drained, 0);
-      }
+      commit_leader(&sm.drained);  // no product may be under way when the CTAs go
+      tc::mbar_wait_drain(&sm.drained, 0);
     }
     __syncwarp();
   } else {
@@ -552,8 +561,31 @@ pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUte
       }
     }
   }
+  if (lane == 0 && *abort)
+    for (int r = 0; r < 2; ++r) st_cluster_i(map_rank(tc::smem_u32(&sm.gave_up), r), 1);
   __syncwarp();
-  cluster_sync();  // the pair's products and copies are done on both sides
+  cluster_sync();  // the pair's products are done on both sides, and its copies if no wait gave up
+  if (sm.gave_up) {
+    // Both CTAs' copies must have landed before either leaves.  The leader's barriers count both, so
+    // the one that has asked for fewer stages first asks for those that the other has asked for:
+    // they are free, since the other one's wait for them ended (their contents are not used).
+    if (threadIdx.x == 0) {
+      const int mine = sm.filled, wanted = max(mine, ld_cluster_i(map_rank(tc::smem_u32(&sm.filled), rank ^ 1)));
+      const uint32_t leader_full = map_rank(tc::smem_u32(&full[0]), 0);
+      for (int k = mine; k < wanted; ++k) {
+        const int st = k % kPairStages;
+        const uint32_t sa = tc::smem_u32(ring) + st * kPairStageBytes;
+        if (rank == 0) tc::mbar_arrive_expect_tx(&full[st], 2 * kPairStageBytes);
+        tma_load_pair(sa, &mx, leader_full + st * 8, 0, 0);
+        tma_load_pair(sa + kTileBytes, &mw, leader_full + st * 8, 0, 0);
+      }
+      if (rank == 0)
+        for (int k = max(wanted - kPairStages, 0); k < wanted; ++k)
+          tc::mbar_wait_drain(&full[k % kPairStages], (k / kPairStages) & 1);
+    }
+    __syncwarp();
+    cluster_sync();
+  }
   if (warp == 1) {
     tc::tc_fence_after();
     tmem_dealloc_pair(tmem, 2 * kPairN);

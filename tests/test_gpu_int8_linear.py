@@ -182,6 +182,41 @@ def test_expired_wait_is_reported():
         assert torch.equal(int8_linear(x, w, None, F32), want)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 2048, 2048), (4, 300, 256), (33, 700, 4096), (64, 4096, 2048), (128, 2048, 8192),
+                                   (300, 1000, 1024), (1500, 1500, 512), (2100, 3000, 3001), (9000, 700, 100)])
+def test_waits_that_run_out_while_copies_are_under_way(M, N, K):
+    """Limits of a few polls: waits give up early or late, with tile loads and products on their way, and
+    once with no load at all.  Each output is NaN or right, and the next call is right: the kernel has
+    waited for its copies and products and given its TMEM back."""
+    from race_attention_b200 import Int8Rows, _lib, int8_linear
+    lib = _lib.load()
+    g = _gen(M + N + K + 1)
+    x, w = Int8Rows(*_rows(g, M, K)), Int8Rows(*_rows(g, N, K))
+    want = int8_linear(x, w, None, F32)
+    gave_up = 0
+    for polls, withhold in [(n, 0) for n in (1, 2, 4, 8, 16, 32, 64, 128, 256)] + [(64, 1)]:
+        lib.race_set_wait_limit(polls)
+        lib.race_test_withhold_first_load(withhold)
+        lib.race_set_status_check(0)
+        try:
+            outs = [int8_linear(x, w, None, F32) for _ in range(3)]
+            torch.cuda.synchronize()
+        finally:
+            lib.race_set_wait_limit(0)
+            lib.race_test_withhold_first_load(0)
+            lib.race_set_status_check(1)
+        expired = any(bool(o.isnan().any()) for o in outs)
+        gave_up += expired
+        assert all(bool((o.isnan() | (o == want)).all()) for o in outs)
+        if withhold:
+            assert all(bool(o.isnan().all()) for o in outs)
+        if expired:  # said once, by the next call that asks
+            with pytest.raises(RuntimeError, match="wait"):
+                int8_linear(x, w, None, F32)
+        assert torch.equal(int8_linear(x, w, None, F32), want)
+    assert gave_up
+
+
 def test_refusals():
     from race_attention_b200 import Int8Rows, int8_linear
     q = torch.zeros(4, 64, dtype=torch.int8, device="cuda")
