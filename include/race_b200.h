@@ -379,7 +379,8 @@ int race_ace_bwd(const void *Q, const void *K, const void *V, const void *dO, in
  * Tensors are rows of `dtype` values (RACE_F32/RACE_BF16) with unit stride inside a
  * row.  Inputs may have any row stride (in elements) of at least the row's length;
  * outputs are dense except 8-bit rows.  All arithmetic is fp32, rounded once into
- * the output's type.  Two calls may run at the same time on different outputs. */
+ * the output's type.  Every array starts at a multiple of its values' size (else
+ * RACE_ERR_ALIGN).  Two calls may run at the same time on different outputs. */
 
 /* h = x + residual, rounded to dtype;  y = h * rsqrt(mean(h^2) + eps) * weight.
  * residual may be NULL (h is x; nothing is written to h, which may be NULL).  weight

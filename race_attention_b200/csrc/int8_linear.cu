@@ -705,7 +705,8 @@ int race_int8_linear(const int8_t *xq, int64_t x_stride, const float *x_scale, c
   if (((reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(wq) | (uintptr_t)x_stride | (uintptr_t)w_stride) & 15) ||
       ((reinterpret_cast<uintptr_t>(x_scale) | reinterpret_cast<uintptr_t>(w_scale) | reinterpret_cast<uintptr_t>(bias)) & 3))
     return err(RACE_ERR_ALIGN, "race_int8_linear: 8-bit rows must start at multiples of 16 bytes");
-  const int size = dtype == RACE_BF16 ? 2 : 4;
+  const int size = race::value_size(dtype);
+  if (const int rc = race::check_values("race_int8_linear", {{y, size}})) return rc;
   Args a{x_scale, w_scale, bias, y, (int)M, (int)N, (int)((K + kBK - 1) / kBK), 0, 0,
          (N * size) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0, race::withhold_first_load() ? 1 : 0,
          race::current_wait_limit()};

@@ -6,6 +6,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <initializer_list>
+
 #include "race_b200.h"
 
 namespace race {
@@ -34,6 +36,22 @@ inline int cuda_err(const char *what, cudaError_t e) {
   snprintf(buf, sizeof(buf), "%s: %s", what, cudaGetErrorString(e));
   return report_error(RACE_ERR_CUDA, buf);
 }
+// RACE_ERR_ALIGN where an array does not start at a multiple of its values' size (no access of a
+// kernel to it would be aligned); absent arrays are NULL.
+struct Values {
+  const void *at;
+  int size;  // of a value, in bytes
+};
+inline int check_values(const char *what, std::initializer_list<Values> arrays) {
+  char buf[160];
+  for (const Values &v : arrays)
+    if (reinterpret_cast<uintptr_t>(v.at) % (uintptr_t)v.size) {
+      snprintf(buf, sizeof(buf), "%s: a tensor does not start at a multiple of its values' size", what);
+      return report_error(RACE_ERR_ALIGN, buf);
+    }
+  return RACE_OK;
+}
+inline int value_size(int dtype) { return dtype == RACE_F32 ? 4 : 2; }
 // Launch of a kernel that starts with wait_for_predecessor(): with the stream's previous kernel
 // still running (once all of its blocks are past let_successor_start(), or done), so that its
 // launch and whatever it does before that call overlap it.

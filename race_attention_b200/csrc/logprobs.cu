@@ -671,12 +671,6 @@ int check_shape(int64_t rows, int64_t V, int64_t stride, int dtype, float temper
   return RACE_OK;
 }
 
-int check_align(int dtype, const void *values) {
-  if (reinterpret_cast<uintptr_t>(values) % (dtype == RACE_F32 ? 4 : 2))
-    return err(RACE_ERR_ALIGN, "token log probabilities: a tensor does not start at a multiple of its values' size");
-  return RACE_OK;
-}
-
 }  // namespace
 
 extern "C" {
@@ -690,7 +684,9 @@ int race_token_logprobs_fwd(const void *logits, int64_t stride, int dtype, const
   if (const int rc = check_shape(rows, V, stride, dtype, temperature)) return rc;
   if (n_top < 0 || n_top > kMaxTop || n_top > V)
     return err(RACE_ERR_SHAPE, "race_token_logprobs_fwd: %lld alternatives (at most %lld, and the vocabulary)", n_top, kMaxTop);
-  if (const int rc = check_align(dtype, logits)) return rc;
+  if (const int rc = race::check_values("race_token_logprobs_fwd", {{logits, race::value_size(dtype)}, {tokens, 8}, {logp, 4}, {entropy, 4},
+                                                                    {n_top ? top_ids : nullptr, 8}, {n_top ? top_logp : nullptr, 4}}))
+    return rc;
   FwdArgs a{logits, tokens, logp, entropy, top_logp, reinterpret_cast<float2 *>(lse), top_ids, stride, ignore_index, rows, (int)V, n_top,
             kLog2e / temperature, 1.f / temperature};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -703,8 +699,10 @@ int race_token_logprobs_bwd(const void *logits, int64_t stride, int dtype, const
   if (!logits || !tokens || !lse || !entropy || !dlogits) return err(RACE_ERR_ARG, "race_token_logprobs_bwd: null pointer");
   if (reinterpret_cast<uintptr_t>(lse) & 7) return err(RACE_ERR_ALIGN, "race_token_logprobs_bwd: lse must be 8-byte aligned");
   if (const int rc = check_shape(rows, V, stride, dtype, temperature)) return rc;
-  if (const int rc = check_align(dtype, logits)) return rc;
-  if (const int rc = check_align(dtype, dlogits)) return rc;
+  const int size = race::value_size(dtype);
+  if (const int rc = race::check_values("race_token_logprobs_bwd", {{logits, size}, {dlogits, size}, {tokens, 8}, {entropy, 4}, {g_logp, 4},
+                                                                    {g_entropy, 4}}))
+    return rc;
   BwdArgs a{logits, tokens, reinterpret_cast<const float2 *>(lse), entropy, g_logp, g_entropy, dlogits, stride, ignore_index,
             rows, (int)V, kLog2e / temperature, 1.f / temperature};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -20,17 +20,17 @@
 #include <math.h>
 #include <stdio.h>
 
-#include <initializer_list>
-
 #include "common.cuh"
 #include "internal.h"
 
 namespace {
 
+using race::check_values;
 using race::err;
 using race::from_f;
 using race::launched;
 using race::to_f;
+using race::value_size;
 
 constexpr int kNT = 256;  // threads of a block that owns one row
 
@@ -829,7 +829,7 @@ __global__ void __launch_bounds__(256) dequant_kernel(const int8_t *q_rows, long
 }
 
 // ------------------------------------------------------------------ host side
-int check_rows(const char *what, int64_t rows, int64_t K, int dtype, std::initializer_list<const void *> values = {}) {
+int check_rows(const char *what, int64_t rows, int64_t K, int dtype) {
   char buf[160];
   if (dtype != RACE_F32 && dtype != RACE_BF16) {
     snprintf(buf, sizeof(buf), "%s: dtype %d", what, dtype);
@@ -840,11 +840,6 @@ int check_rows(const char *what, int64_t rows, int64_t K, int dtype, std::initia
     snprintf(buf, sizeof(buf), "%s: rows=%lld (1..2^31-1), width=%lld (1..2^24)", what, (long long)rows, (long long)K);
     return race::report_error(RACE_ERR_SHAPE, buf);
   }
-  for (const void *p : values)
-    if (reinterpret_cast<uintptr_t>(p) % (dtype == RACE_F32 ? 4 : 2)) {
-      snprintf(buf, sizeof(buf), "%s: a tensor does not start at a multiple of its values' size", what);
-      return race::report_error(RACE_ERR_ALIGN, buf);
-    }
   return RACE_OK;
 }
 
@@ -989,10 +984,12 @@ int race_rms_norm_fwd(const void *x, int64_t x_stride, const void *residual, int
                       const void *weight, int weight_dtype, void *y, void *h, float *rstd, int64_t rows, int64_t K,
                       float eps, void *stream) {
   if (!x || !y || (residual && !h)) return err(RACE_ERR_ARG, "race_rms_norm_fwd: null pointer");
-  if (const int rc = check_rows("race_rms_norm_fwd", rows, K, dtype, {x, residual, y, h})) return rc;
+  if (const int rc = check_rows("race_rms_norm_fwd", rows, K, dtype)) return rc;
   if (weight && weight_dtype != RACE_F32 && weight_dtype != RACE_BF16)
     return err(RACE_ERR_DTYPE, "race_rms_norm_fwd: weight dtype %lld", weight_dtype);
   if (x_stride < K || (residual && residual_stride < K)) return err(RACE_ERR_SHAPE, "race_rms_norm_fwd: row stride below the width %lld", K);
+  const int size = value_size(dtype), w_size = weight ? value_size(weight_dtype) : 1;
+  if (const int rc = check_values("race_rms_norm_fwd", {{x, size}, {residual, size}, {y, size}, {h, size}, {weight, w_size}, {rstd, 4}})) return rc;
   RowArgs a{x, residual, weight, y, h, nullptr, nullptr, rstd, rows, x_stride, residual_stride, 0, (int)K, weight_dtype == RACE_BF16, eps};
   return launch_rows<kNorm>("rms_norm_fwd", a, dtype, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -1001,11 +998,13 @@ int race_rms_norm_int8(const void *x, int64_t x_stride, const void *residual, in
                        const void *weight, int weight_dtype, int8_t *q, int64_t q_stride, float *scale, void *h,
                        int64_t rows, int64_t K, float eps, void *stream) {
   if (!x || !q || !scale || (residual && !h)) return err(RACE_ERR_ARG, "race_rms_norm_int8: null pointer");
-  if (const int rc = check_rows("race_rms_norm_int8", rows, K, dtype, {x, residual, h})) return rc;
+  if (const int rc = check_rows("race_rms_norm_int8", rows, K, dtype)) return rc;
   if (weight && weight_dtype != RACE_F32 && weight_dtype != RACE_BF16)
     return err(RACE_ERR_DTYPE, "race_rms_norm_int8: weight dtype %lld", weight_dtype);
   if (x_stride < K || q_stride < K || (residual && residual_stride < K))
     return err(RACE_ERR_SHAPE, "race_rms_norm_int8: row stride below the width %lld", K);
+  const int size = value_size(dtype), w_size = weight ? value_size(weight_dtype) : 1;
+  if (const int rc = check_values("race_rms_norm_int8", {{x, size}, {residual, size}, {h, size}, {weight, w_size}, {scale, 4}})) return rc;
   RowArgs a{x, residual, weight, nullptr, h, q, scale, nullptr, rows, x_stride, residual_stride, q_stride, (int)K, weight_dtype == RACE_BF16, eps};
   return launch_rows<kNormInt8>("rms_norm_int8", a, dtype, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -1013,8 +1012,9 @@ int race_rms_norm_int8(const void *x, int64_t x_stride, const void *residual, in
 int race_quant_int8(const void *x, int64_t x_stride, int dtype, int8_t *q, int64_t q_stride, float *scale, int64_t rows,
                     int64_t K, void *stream) {
   if (!x || !q || !scale) return err(RACE_ERR_ARG, "race_quant_int8: null pointer");
-  if (const int rc = check_rows("race_quant_int8", rows, K, dtype, {x})) return rc;
+  if (const int rc = check_rows("race_quant_int8", rows, K, dtype)) return rc;
   if (x_stride < K || q_stride < K) return err(RACE_ERR_SHAPE, "race_quant_int8: row stride below the width %lld", K);
+  if (const int rc = check_values("race_quant_int8", {{x, value_size(dtype)}, {scale, 4}})) return rc;
   RowArgs a{x, nullptr, nullptr, nullptr, nullptr, q, scale, nullptr, rows, x_stride, 0, q_stride, (int)K, 0, 0.f};
   return launch_rows<kQuantInt8>("quant_int8", a, dtype, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -1022,8 +1022,9 @@ int race_quant_int8(const void *x, int64_t x_stride, int dtype, int8_t *q, int64
 int race_swiglu_int8(const void *gate_up, int64_t stride, int dtype, int8_t *q, int64_t q_stride, float *scale,
                      int64_t rows, int64_t F, void *stream) {
   if (!gate_up || !q || !scale) return err(RACE_ERR_ARG, "race_swiglu_int8: null pointer");
-  if (const int rc = check_rows("race_swiglu_int8", rows, F, dtype, {gate_up})) return rc;
+  if (const int rc = check_rows("race_swiglu_int8", rows, F, dtype)) return rc;
   if (stride < 2 * F || q_stride < F) return err(RACE_ERR_SHAPE, "race_swiglu_int8: row stride below the width (F=%lld)", F);
+  if (const int rc = check_values("race_swiglu_int8", {{gate_up, value_size(dtype)}, {scale, 4}})) return rc;
   RowArgs a{gate_up, nullptr, nullptr, nullptr, nullptr, q, scale, nullptr, rows, stride, 0, q_stride, (int)F, 0, 0.f};
   return launch_rows<kSwigluInt8>("swiglu_int8", a, dtype, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -1031,8 +1032,9 @@ int race_swiglu_int8(const void *gate_up, int64_t stride, int dtype, int8_t *q, 
 int race_dequant_int8(const int8_t *q, int64_t q_stride, const float *scale, void *out, int dtype, int64_t rows,
                       int64_t K, void *stream) {
   if (!q || !scale || !out) return err(RACE_ERR_ARG, "race_dequant_int8: null pointer");
-  if (const int rc = check_rows("race_dequant_int8", rows, K, dtype, {out})) return rc;
+  if (const int rc = check_rows("race_dequant_int8", rows, K, dtype)) return rc;
   if (q_stride < K) return err(RACE_ERR_SHAPE, "race_dequant_int8: row stride below the width %lld", K);
+  if (const int rc = check_values("race_dequant_int8", {{out, value_size(dtype)}, {scale, 4}})) return rc;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // rows of up to 2048 values share a block of 256 threads
   int x = 1;
@@ -1070,11 +1072,15 @@ int race_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float
                       int weight_dtype, void *dx, void *dw, int64_t rows, int64_t K, void *workspace,
                       size_t workspace_bytes, void *stream) {
   if (!dy || !h || !rstd || !dx) return err(RACE_ERR_ARG, "race_rms_norm_bwd: null pointer");
-  if (const int rc = check_rows("race_rms_norm_bwd", rows, K, dtype, {dy, dh, h, dx})) return rc;
+  if (const int rc = check_rows("race_rms_norm_bwd", rows, K, dtype)) return rc;
   if ((weight || dw) && weight_dtype != RACE_F32 && weight_dtype != RACE_BF16)
     return err(RACE_ERR_DTYPE, "race_rms_norm_bwd: weight dtype %lld", weight_dtype);
   if (dw && (!workspace || workspace_bytes < race_rms_norm_bwd_workspace_bytes(rows, K)))
     return err(RACE_ERR_WORKSPACE, "race_rms_norm_bwd: workspace of %lld bytes needed", (long long)race_rms_norm_bwd_workspace_bytes(rows, K));
+  const int size = value_size(dtype), w_size = weight || dw ? value_size(weight_dtype) : 1;
+  if (const int rc = check_values("race_rms_norm_bwd", {{dy, size}, {dh, size}, {h, size}, {dx, size}, {rstd, 4}, {weight, w_size},
+                                                        {dw, w_size}, {dw ? workspace : nullptr, 4}}))
+    return rc;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int blocks = bwd_blocks(rows, K);
   BwdArgs a{dy, dh, h, weight, rstd, dx, dw, dw ? static_cast<float *>(workspace) : nullptr, rows, (int)K, weight_dtype == RACE_BF16};

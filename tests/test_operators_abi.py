@@ -89,6 +89,32 @@ def test_strides_and_weights():
     assert norm_bwd(ws=None) == norm_bwd(nb=need - 1) == "RACE_ERR_WORKSPACE"
 
 
+def _at(n):
+    return ctypes.c_void_p(256 + n)
+
+
+@pytest.mark.parametrize("call,arrays", [
+    (norm_fwd, dict(x=4, r=4, w=4, y=4, h=4, rstd=4)), (norm_int8, dict(x=4, r=4, w=4, s=4, h=4)),
+    (norm_bwd, dict(dy=4, h=4, rstd=4, w=4, dx=4, dw=4, ws=4)), (quant, dict(x=4, s=4)), (swiglu, dict(x=4, s=4)),
+    (dequant, dict(s=4, o=4)), (linear, dict(s=4, t=4, b=4, y=4)),
+    (logp_fwd, dict(l=4, t=8, lp=4, e=4, lse=8, ids=8, top=4)), (logp_bwd, dict(l=4, t=8, lse=8, e=4, d=4)),
+])
+def test_arrays_that_start_inside_a_value(call, arrays):
+    for name, size in arrays.items():
+        for n in (1, size // 2):
+            assert call(**{name: _at(n)}) == "RACE_ERR_ALIGN", (name, n)
+
+
+def test_arrays_of_bf16_that_start_inside_a_value():
+    for call, names in ((norm_fwd, "x r y h"), (norm_int8, "x r h"), (norm_bwd, "dy h dx"), (quant, "x"), (swiglu, "x"),
+                        (dequant, "o"), (linear, "y"), (logp_fwd, "l"), (logp_bwd, "l d")):
+        for name in names.split():
+            assert call(dt=BF16, **{name: _at(1)}) == "RACE_ERR_ALIGN", name
+    for call in (norm_fwd, norm_int8, norm_bwd):
+        assert call(w=_at(1), wd=BF16) == "RACE_ERR_ALIGN"
+    assert norm_bwd(w=None, dw=_at(1), wd=BF16) == "RACE_ERR_ALIGN"
+
+
 def test_linear():
     assert linear(M=0) == linear(N=0) == linear(K=0) == linear(K=131072) == linear(M=1 << 31) == "RACE_ERR_SHAPE"
     assert linear(xs=48) == linear(ws=48) == "RACE_ERR_SHAPE"
