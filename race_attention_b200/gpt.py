@@ -39,11 +39,15 @@ class GPTConfig:
     race_eps: float = 1e-6
     rope_base: float = 10000.0
     fused: bool = False        # add_rms_norm in the blocks, token_logprobs for the loss
-    norm_eps: float = 1e-6     # of the fused norms
+    norm_eps: float | None = None  # of every norm, fused or not; None: torch's default, fp32's epsilon
+
+    @property
+    def fused_norm_eps(self):
+        return torch.finfo(torch.float32).eps if self.norm_eps is None else self.norm_eps
 
 
-def _rms(x):
-    return F.rms_norm(x, (x.size(-1),))
+def _rms(x, eps):
+    return F.rms_norm(x, (x.size(-1),), eps=eps)
 
 
 class _Linear(nn.Linear):
@@ -78,7 +82,8 @@ class RaceAttention(nn.Module):
         q = self.c_q(x).view(B, T, self.n_head, self.head_dim)
         k = self.c_k(x).view(B, T, self.n_head, self.head_dim)
         v = self.c_v(x).view(B, T, self.n_head, self.head_dim)
-        q, k = _rms(_rotary(q, cos, sin)) * 1.2, _rms(_rotary(k, cos, sin)) * 1.2  # QK norm, sharpened
+        eps = self.cfg.norm_eps
+        q, k = _rms(_rotary(q, cos, sin), eps) * 1.2, _rms(_rotary(k, cos, sin), eps) * 1.2  # QK norm, sharpened
         y = nanochat_race_attention(q, k, v, self.planes_T, self.cfg.race_L, self.cfg.race_P, 1, self.cfg.race_eps)
         return self.c_proj(y.reshape(B, T, C))
 
@@ -96,16 +101,19 @@ class MLP(nn.Module):
 class Block(nn.Module):
     def __init__(self, cfg: GPTConfig, layer_idx: int):
         super().__init__()
+        self.cfg = cfg
         self.attn = RaceAttention(cfg, layer_idx)
         self.mlp = MLP(cfg)
 
     def forward(self, x, cos, sin):
-        x = x + self.attn(_rms(x), cos, sin)
-        return x + self.mlp(_rms(x))
+        eps = self.cfg.norm_eps
+        x = x + self.attn(_rms(x, eps), cos, sin)
+        return x + self.mlp(_rms(x, eps))
 
-    def forward_fused(self, d, x, cos, sin, eps):
+    def forward_fused(self, d, x, cos, sin):
         """The residual stream x and what is still to be added to it (d, None in front of the first
         block), to both after the block."""
+        eps = self.cfg.fused_norm_eps
         y, x = add_rms_norm(x, None, None, eps) if d is None else add_rms_norm(d, x, None, eps)
         y, x = add_rms_norm(self.attn(y, cos, sin), x, None, eps)
         return self.mlp(y), x
@@ -132,15 +140,15 @@ class RaceGPT(nn.Module):
     def logits(self, idx, dtype=torch.bfloat16):
         B, T = idx.shape
         cos, sin = self._angles(T, idx.device, dtype)
-        x = _rms(self.wte(idx).to(dtype))
+        x = _rms(self.wte(idx).to(dtype), self.cfg.norm_eps)
         if self.cfg.fused:
             d = None
             for blk in self.blocks:
-                d, x = blk.forward_fused(d, x, cos, sin, self.cfg.norm_eps)
-            return self.lm_head(add_rms_norm(d, x, None, self.cfg.norm_eps)[0])
+                d, x = blk.forward_fused(d, x, cos, sin)
+            return self.lm_head(add_rms_norm(d, x, None, self.cfg.fused_norm_eps)[0])
         for blk in self.blocks:
             x = blk(x, cos, sin)
-        return self.lm_head(_rms(x))
+        return self.lm_head(_rms(x, self.cfg.norm_eps))
 
     def token_logprobs(self, idx, targets, temperature=1.0, n_top=0, dtype=torch.bfloat16):
         """TokenLogprobs of targets [B, T] (-100: none) after idx [B, T], differentiable."""

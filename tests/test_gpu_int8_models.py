@@ -122,6 +122,34 @@ def test_gpt_fused_matches_the_plain_harness():
         assert err < 5e-2, (name, err)
 
 
+@pytest.mark.parametrize("norm_eps", [None, 1e-6, 1e-2])
+def test_gpt_fused_norms_take_the_plain_ones_eps(norm_eps):
+    """A residual stream whose mean square is near the smaller of these eps, one block and the whole model:
+    both forms agree within the bf16 tolerance (5e-2 by 2-norm), where another eps is 20 % off or more."""
+    from race_attention_b200.gpt import GPTConfig, RaceGPT
+    outs = []
+    for fused in (False, True):
+        torch.manual_seed(0)
+        cfg = GPTConfig(vocab_size=509, n_layer=2, n_head=2, n_embd=128, mlp_hidden=256, race_L=8, fused=fused,
+                        norm_eps=norm_eps)
+        model = RaceGPT(cfg).cuda()
+        model.init_weights(0.05)
+        g = torch.Generator(device="cuda").manual_seed(5)
+        x = (torch.randn(1, 200, 128, device="cuda", generator=g) * 1e-3).bfloat16()
+        idx = torch.randint(0, 509, (1, 200), device="cuda", generator=g)
+        with torch.no_grad():
+            cos, sin = model._angles(200, x.device, x.dtype)
+            if fused:
+                d, h = model.blocks[0].forward_fused(None, x, cos, sin)
+                y = d.float() + h.float()
+            else:
+                y = model.blocks[0](x, cos, sin).float()
+            model.wte.weight.mul_(0.02)
+            outs.append((y, model(idx).float()))
+    for a, b in zip(*outs):
+        assert float((a - b).norm() / a.norm()) < 5e-2
+
+
 def test_gpt_policy_gradient_steps():
     """A few steps on log probabilities weighted by advantages with an entropy bonus: the sampled
     tokens with positive advantages become more probable than those with negative ones."""
