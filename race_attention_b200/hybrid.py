@@ -90,6 +90,8 @@ class Layer(nn.Module):
         self.int8 = False
 
     def quantize_int8(self):
+        if self.int8:
+            return
         self.qkv, self.o, self.gate_up, self.down = (Int8Linear.from_linear(m) for m in
                                                      (self.qkv, self.o, self.gate_up, self.down))
         self.int8 = True
@@ -199,10 +201,12 @@ class HybridLlama(nn.Module):
 
     @torch.no_grad()
     def quantize_int8(self):
-        """Projections, MLP and LM head as 8-bit layers, in place (the embedding stays as it is)."""
+        """Projections, MLP and LM head as 8-bit layers, in place (the embedding stays as it is).
+        What is in 8 bits already is left alone."""
         for layer in self.layers:
             layer.quantize_int8()
-        self.head = Int8Linear(self.embed.weight, dtype=self.embed.weight.dtype)
+        if self.head is None:
+            self.head = Int8Linear(self.embed.weight, dtype=self.embed.weight.dtype)
         return self
 
     def _logits(self, x):

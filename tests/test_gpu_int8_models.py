@@ -69,6 +69,16 @@ def test_int8_decode_graph_replays_the_eager_steps():
         assert torch.equal(ta, tb)
 
 
+def test_quantising_twice_changes_nothing():
+    _, model = _hybrid()
+    model.quantize_int8()
+    before = [m for m in model.modules()]
+    held = {k: v.clone() for k, v in model.state_dict().items()}
+    assert model.quantize_int8() is model
+    assert all(a is b for a, b in zip(before, model.modules(), strict=True))
+    assert all(torch.equal(held[k], v) for k, v in model.state_dict().items())
+
+
 @pytest.mark.parametrize("int8", [False, True])
 def test_answers_with_log_probabilities(int8):
     cfg, model = _hybrid(3)
