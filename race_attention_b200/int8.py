@@ -83,9 +83,12 @@ class Int8Linear(nn.Module):
         return cls(linear.weight, linear.bias, linear.weight.dtype)
 
     def _apply(self, fn, *args, **kwargs):
-        held = self.scale, self.bias
+        held = {"scale": self.scale, "bias": self.bias}
         super()._apply(fn, *args, **kwargs)
-        self.scale, self.bias = (None if t is None else t.to(self.q.device) for t in held)
+        for name, t in held.items():
+            moved = getattr(self, name)
+            if t is not None and moved.dtype != t.dtype:
+                setattr(self, name, t.to(moved.device))
         return self
 
     def forward(self, x):

@@ -1,0 +1,34 @@
+"""Host-side behaviour of the models and layers around the RACE layer (runs without a GPU)."""
+import torch
+
+
+def _int8_linear():
+    """An Int8Linear of given rows (its constructor quantises on the GPU)."""
+    from race_attention_b200 import Int8Linear
+    layer = Int8Linear.__new__(Int8Linear)
+    torch.nn.Module.__init__(layer)
+    layer.out_features, layer.in_features, layer.dtype = 3, 16, torch.bfloat16
+    layer.register_buffer("q", torch.arange(48, dtype=torch.int8).view(3, 16))
+    layer.register_buffer("scale", torch.tensor([0.1, 0.3, 1 / 3]))
+    layer.register_buffer("bias", torch.tensor([0.7, -0.1, 1 / 7]))
+    return layer
+
+
+def test_int8_layer_keeps_its_scales_when_converted():
+    layer = _int8_linear()
+    want = {k: v.clone() for k, v in layer.state_dict().items()}
+    for kind in (torch.bfloat16, torch.float16, torch.float64, torch.float32):
+        moved = layer.to(kind)
+        assert moved is layer
+        assert all(torch.equal(want[k], v) and want[k].dtype == v.dtype for k, v in layer.state_dict().items())
+
+
+def test_int8_layer_leaves_the_meta_device():
+    layer = _int8_linear()
+    held = {k: v.clone() for k, v in layer.state_dict().items()}
+    layer.to(torch.bfloat16).to("meta")
+    assert all(v.device.type == "meta" for v in layer.state_dict().values())
+    layer.to_empty(device="cpu")
+    layer.load_state_dict(held)
+    assert all(torch.equal(held[k], v) and held[k].dtype == v.dtype for k, v in layer.state_dict().items())
+    assert layer.q.device.type == layer.scale.device.type == layer.bias.device.type == "cpu"
