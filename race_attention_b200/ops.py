@@ -516,19 +516,17 @@ def gqa_decode_attention(q, k_new, v_new, k_cache, v_cache, length, workspace, n
 # probabilities.  Some of them run for a few microseconds on a decode step, so their checks
 # are single passes over attributes and they launch without entering a device context where
 # the tensors' device is current.
-_current_device = torch._C._cuda_getDevice
-_current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _launch(dev, name, *args):
     """Call C entry point `name` with args and the current stream of `dev`."""
     fn = getattr(_lib.load(), name)
     index = dev.index
-    if index == _current_device():
-        rc = fn(*args, _current_stream(index))
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _current_stream(index))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, name)
 

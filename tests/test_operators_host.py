@@ -1,5 +1,10 @@
 """Host-side behaviour of the models and layers around the RACE layer (runs without a GPU)."""
+import subprocess
+import sys
+
 import torch
+
+from conftest import ROOT
 
 
 def _int8_linear():
@@ -32,3 +37,17 @@ def test_int8_layer_leaves_the_meta_device():
     layer.load_state_dict(held)
     assert all(torch.equal(held[k], v) and held[k].dtype == v.dtype for k, v in layer.state_dict().items())
     assert layer.q.device.type == layer.scale.device.type == layer.bias.device.type == "cpu"
+
+
+def test_package_imports_where_torch_has_no_cuda():
+    """What needs no GPU (planes, the host's part of the shard exchange) works with a torch built without CUDA."""
+    code = """
+import torch
+for name in [n for n in dir(torch._C) if n.startswith("_cuda_get")]:
+    delattr(torch._C, name)
+import race_attention_b200 as rb
+planes, _ = rb.build_planes_protos(64, 4, 16, 1, device="cpu", seed=0)
+assert planes.isfinite().all()
+"""
+    run = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
