@@ -241,8 +241,8 @@ class HybridLlama(nn.Module):
         cos, sin = self._angles(0, T, idx.device, self.embed.weight.dtype)
         nxt = []
         for b0 in range(0, B, micro_batch):
-            logits = self._prefill_hidden(self.embed(idx[b0:b0 + micro_batch]), cos, sin, t_max, b0, B)
-            nxt.append(logits(-1).argmax(-1))
+            # (unnamed: nothing of a slice is held while the next one is worked on)
+            nxt.append(self._prefill_hidden(self.embed(idx[b0:b0 + micro_batch]), cos, sin, t_max, b0, B)(-1).argmax(-1))
         self.pos = torch.full((1,), T, dtype=torch.int32, device=idx.device)
         self.n_tokens, self.t_max = T, t_max
         return torch.cat(nxt)

@@ -1,6 +1,7 @@
 """Host-side behaviour of the models and layers around the RACE layer (runs without a GPU)."""
 import subprocess
 import sys
+import weakref
 
 import torch
 
@@ -51,3 +52,23 @@ assert planes.isfinite().all()
 """
     run = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr
+
+
+def _hybrid():
+    from race_attention_b200.hybrid import HybridConfig, HybridLlama
+    torch.manual_seed(0)
+    return HybridLlama(HybridConfig(vocab_size=50, n_layer=2, hidden=64, n_head=2, n_kv_head=1, mlp_hidden=64))
+
+
+def test_prefill_lets_go_of_each_slice(monkeypatch):
+    """No hidden state of one slice of the batch is held while the next one is worked on."""
+    model, seen = _hybrid(), []
+
+    def hidden(x, cos, sin, t_max, b0, batch):
+        assert not any(r() is not None for r in seen), "an earlier slice is still held"
+        seen.append(weakref.ref(x))
+        return lambda at: x[:, at]
+
+    monkeypatch.setattr(model, "_prefill_hidden", hidden)
+    assert model.prefill(torch.zeros(6, 5, dtype=torch.int64), t_max=8, micro_batch=2).shape == (6,)
+    assert len(seen) == 3
