@@ -228,10 +228,11 @@ class HybridLlama(nn.Module):
         B, T = idx.shape
         kept = [(layer.state, layer.cache, layer.attn_ws, layer.n_splits) for layer in self.layers]
         cos, sin = self._angles(0, T, idx.device, self.embed.weight.dtype)
-        logits = self._prefill_hidden(self.embed(idx), cos, sin, T, 0, B)
-        for layer, (st, cache, ws, ns) in zip(self.layers, kept):
-            layer.state, layer.cache, layer.attn_ws, layer.n_splits = st, cache, ws, ns
-        return logits
+        try:
+            return self._prefill_hidden(self.embed(idx), cos, sin, T, 0, B)
+        finally:
+            for layer, (st, cache, ws, ns) in zip(self.layers, kept):
+                layer.state, layer.cache, layer.attn_ws, layer.n_splits = st, cache, ws, ns
 
     @torch.no_grad()
     def prefill(self, idx, t_max, micro_batch=4):

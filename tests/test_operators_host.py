@@ -3,6 +3,7 @@ import subprocess
 import sys
 import weakref
 
+import pytest
 import torch
 
 from conftest import ROOT
@@ -72,3 +73,26 @@ def test_prefill_lets_go_of_each_slice(monkeypatch):
     monkeypatch.setattr(model, "_prefill_hidden", hidden)
     assert model.prefill(torch.zeros(6, 5, dtype=torch.int64), t_max=8, micro_batch=2).shape == (6,)
     assert len(seen) == 3
+
+
+def test_scoring_that_fails_leaves_the_decode_state(monkeypatch):
+    """A forward that stops half-way (out of memory, say) leaves every layer's state and cache as they were."""
+    model = _hybrid()
+    for layer in model.layers:
+        layer.state, layer.cache, layer.attn_ws, layer.n_splits = object(), (object(), object()), object(), 7
+    held = [(a.state, a.cache, a.attn_ws, a.n_splits) for a in model.layers]
+
+    def first(x, cos, sin, t_max, b0, batch):
+        layer = model.layers[0]
+        layer.state, layer.cache, layer.attn_ws, layer.n_splits = None, None, None, 1
+        return x
+
+    def second(x, *a):
+        raise RuntimeError("out of memory")
+
+    monkeypatch.setattr(model.layers[0], "prefill", first)
+    monkeypatch.setattr(model.layers[1], "prefill", second)
+    for call in (model.score, model.logits_full):
+        with pytest.raises(RuntimeError, match="out of memory"):
+            call(torch.zeros(2, 5, dtype=torch.int64))
+        assert [(a.state, a.cache, a.attn_ws, a.n_splits) for a in model.layers] == held
