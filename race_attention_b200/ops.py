@@ -515,18 +515,20 @@ def gqa_decode_attention(q, k_new, v_new, k_cache, v_cache, length, workspace, n
 # operators around the layer: residual RMS norm, 8-bit rows and products, token log
 # probabilities.  Some of them run for a few microseconds on a decode step, so their checks
 # are single passes over attributes and they launch without entering a device context where
-# the tensors' device is current.
+# the tensors' device is current.  (None with a torch that has no CUDA: nothing is launched there.)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _launch(dev, name, *args):
     """Call C entry point `name` with args and the current stream of `dev`."""
     fn = getattr(_lib.load(), name)
     index = dev.index
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index == _current_device():
+        rc = fn(*args, _current_stream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(*args, _current_stream(index))
     if rc:
         _lib.check(rc, name)
 
