@@ -625,9 +625,9 @@ int launch_split(const CUtensorMap &mx, const CUtensorMap &mw, const Args &a, cu
   if (e != cudaSuccess) return cuda_err("int8_linear", e);
   const int n_tiles = (a.N + kTileRows - 1) / kTileRows, m_tiles = (a.M + BT - 1) / BT;
   // Split K while each CTA keeps two K steps and the CTAs fit on the SMs at once: two per SM up
-  // to 64 tokens (64 x 16384 x 2048: 12.6 us with 256 CTAs, 13.8 with 128), one with 128, whose
-  // sums to exchange cost more than more CTAs gain (256 x 2048 x 2048: 8.3 us with one per SM,
-  // 18.7 with two; 128 x 2048 x 2048: 8.1 us split four ways, 13.0 eight).
+  // to 64 tokens (64 x 16384 x 2048: 11.4 us with 256 CTAs, 12.8 with 128), one with 128, whose
+  // sums to exchange cost more than more CTAs gain (777 x 1001 x 2050: 10.6 us with one per SM,
+  // 16.4 with two; 128 x 2048 x 2048: 7.1 us split four ways, 11.8 eight).
   const int room = sm_count() * (BT <= 64 ? 2 : 1);
   int S = 1;
   constexpr int kMost = BT <= 64 ? kMaxSplit : kMaxSplit / 2;
@@ -652,8 +652,9 @@ template <typename T>
 int launch(const int8_t *xq, int64_t x_stride, const int8_t *wq, int64_t w_stride, int64_t K, Args a, cudaStream_t s) {
   a.m_tiles = (a.M + 255) / 256;
   a.n_tiles = (a.N + kPairN - 1) / kPairN;
-  // The pair kernel once its tiles occupy a third of the pairs (1024 x 2048 x 2048, 32 tiles: 10.8
-  // us against 13.0 split; 777 x 1001 x 2050, 16 tiles: 13.5 against 10.9).
+  // The pair kernel once its tiles occupy a third of the pairs (1024 x 2048 x 2048, 32 tiles: 11.7
+  // us against 13.8 split; 777 x 1001 x 2050, 16 tiles: 14.9 against 10.6; 1024 x 1024 x 2048, 16
+  // tiles: 10.8 against 9.2).
   const bool pairs = a.M > 128 && (long long)a.m_tiles * a.n_tiles >= sm_count() / 6;
   const int BT = pairs ? 128 : a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
   CUtensorMap mx, mw;

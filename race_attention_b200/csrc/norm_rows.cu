@@ -11,10 +11,9 @@
 //                   correctly rounded
 // Sums, statistics and everything up to the last rounding are fp32.
 //
-// A row of zeros (or of values under 2^-143, whose scale fp32 does not hold) has scale 0 and q = 0.
-// A row that holds a NaN (or whose largest
-// magnitude is infinite) has scale NaN (infinity), so whatever is computed from it
-// is not finite either; no such row touches another.
+// A row of zeros (or of values under 2^-143, whose scale fp32 does not hold) has scale 0 and
+// q = 0.  A row that holds a NaN (or whose largest magnitude is infinite) has scale NaN
+// (infinity), so whatever is computed from it is not finite either; no such row touches another.
 #include "race_b200.h"
 
 #include <math.h>
@@ -431,8 +430,9 @@ __device__ __forceinline__ int group_size() {
 
 // What bounds it is the rows' one trip from and to HBM; see launch_width for the widths' groups
 // and what they measured.
-// Least blocks per SM: what bounds the registers, see launch_width.  Only where that takes no
-// spills (fp32 vectors and skewed rows' weights fill them).
+// Least blocks (of row_block(G) threads) per SM, which bounds the registers: 40 a thread for two
+// vectors, 56 for four.  Only where that takes no spills (fp32 vectors and skewed rows' weights
+// fill them).
 template <typename T, int G, int VPT, int LAYOUT>
 constexpr int row_blocks() {
   return sizeof(T) == 4 || LAYOUT != kAligned ? 0 : G == 512 ? 3 : G == 288 ? (VPT == 4 ? 4 : 5) : 0;
@@ -533,7 +533,10 @@ __global__ void __launch_bounds__(row_block(G), row_blocks<T, G, VPT, LAYOUT>())
   }
 }
 
-// Any width: the row is read again for each of its passes (from the caches).
+// Any width and any layout: the row is read again for each of its passes (from the caches), by
+// single values.  What takes it is rows past the widths below, and a view beside dense tensors whose
+// rows lie otherwise: 32768 x 2048 bf16 with x one value into its rows takes 133 us for the norm and
+// 201 for the 8-bit norm, against 80 and 72 for aligned rows (64 rows: 3.6 and 4.2 against 1.9).
 template <typename T, int MODE>
 __global__ void __launch_bounds__(kNT) row_loop_kernel(RowArgs a) {
   __shared__ float red[32];
@@ -864,9 +867,10 @@ void launch_row_kernel(const RowArgs &a, int vectors, cudaStream_t s) {
 // Threads per row.  A warp up to 1024 values: no barriers, all of a row's loads in flight at
 // once.  Wider rows take a block with two vectors per thread (32768 x 2048 bf16: norm 79 us with
 // 128 threads, 83 with 64, 124 with a warp), four past 4096 values (8192: norm 157 us with 256
-// threads, 171 with 512, 198 with 1024), and blocks of registers few enough for 40 warps per SM
-// (the 8-bit norm's two kernels: 32768 x 2048 80 us without that bound, 70 with it; 16384 x 8192
-// 169 and 136).  Few rows spread each over more threads, for latency.
+// threads, 171 with 512, 198 with 1024).  Their registers are bounded (see row_blocks) to what lets
+// 48 warps onto an SM at 2048 values and 32 at 8192: before its quotients were exact the 8-bit norm of
+// 32768 x 2048 took 80 us without that bound and 70 with it, of 16384 x 8192 169 and 136.  Few rows
+// spread each over more threads, for latency.
 template <typename T, int MODE, int LAYOUT>
 void launch_width(const RowArgs &a, cudaStream_t s) {
   const int n = (a.K + (LAYOUT == kSkewed ? 7 : 0) + 7) / 8;  // vectors, whatever the offset
@@ -924,8 +928,11 @@ int launch_rows(const char *what, const RowArgs &a, int dtype, cudaStream_t s) {
 }
 
 // Blocks of the backward, each with one row of partial sums of dw to be added: four per SM of
-// a B200, two where they hold eight rows at a time (up to 768 values), eight where they are of 64
-// threads; with few rows a row each, then four.  A multiple of 8 (see kSkewed).
+// a B200, two where they hold eight rows at a time (up to 768 values), eight from there to 1024
+// values (blocks of 64 threads where rows are aligned bf16, else of 128).  Few rows: as many blocks
+// up to 148, 148 up to 592 rows, then one for four rows; blocks that hold eight rows at a time leave
+// up to seven eighths of those without a row (1000 rows: 125 of 256 have some, the others add
+// zeros).  A multiple of 8 (see kSkewed).
 int bwd_blocks(int64_t rows, int64_t K) {
   const int64_t n = rows <= 148 ? rows : rows <= 592 ? 148 : (rows + 3) / 4, most = K <= 768 ? 296 : K <= 1024 ? 1184 : 592;
   return (int)(n < most ? (n + 7) / 8 * 8 : most);
@@ -949,6 +956,9 @@ void launch_bwd_width(const BwdArgs &a, int blocks, cudaStream_t s) {
   // against 134, 32768 x 2048 105 against 149); with fp32 or skewed rows they cost registers
   // that the blocks then lack (fp32 32768 x 2048 237 us against 168, bf16 65536 x 1001 196
   // against 138).
+  // Blocks of 320 threads, two per SM, for 257 to 320 vectors: with those of 512, of which an SM's
+  // registers hold one, fp32 20000 x 2047 takes 172 us against 131, 20000 x 2560 159 against 147,
+  // 1000 x 2047 16.2 against 12.8, bf16 20000 x 2047 168 against 111.
   if constexpr (sizeof(T) == 2 && LAYOUT == kAligned) {
     if (n <= 128) return launch_bwd_kernel<T, 64, 2, LAYOUT>(a, blocks, n, s);
     if (n <= 256) return launch_bwd_kernel<T, 128, 2, LAYOUT>(a, blocks, n, s);
