@@ -407,7 +407,10 @@ int race_rms_norm_bwd(const void *dy, const void *dh, const void *h, const float
  *   race_quant_int8:     v = x
  *   race_rms_norm_int8:  v = the y of race_rms_norm_fwd, not rounded in between; h as there
  *   race_swiglu_int8:    v = silu(gate) * up of rows [gate F | up F]
- *   race_dequant_int8:   out[r, k] = q[r, k] * scale[r], rounded to dtype */
+ *   race_dequant_int8:   out[r, k] = q[r, k] * scale[r], rounded to dtype
+ * The norm's v carries the error of fp32 sums (1e-6 or so of itself), SwiGLU's that of approximate
+ * exponentials and reciprocals (2e-6, for gates below -20 up to 1e-5): values that close to half a
+ * step may come out on either side of it. */
 int race_quant_int8(const void *x, int64_t x_stride, int dtype, int8_t *q, int64_t q_stride, float *scale, int64_t rows,
                     int64_t K, void *stream);
 int race_rms_norm_int8(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, int dtype,
