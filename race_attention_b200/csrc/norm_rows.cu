@@ -520,8 +520,8 @@ __global__ void __launch_bounds__(row_block(G), row_blocks<T, G, VPT, LAYOUT>())
       uint2 b[VPT];
       // By pairs of values unless their registers cost a block per SM or spill (bf16: 8-bit norm of
       // 16384 x 8192 139 us by single values and 155 by pairs, rows of 16384 values to 8 bits 193
-      // and 260; elsewhere 16384 x 8192 SwiGLU 104 us by pairs and 108 by single values, 262144 x
-      // 256 to 8 bits 41 and 42).
+      // and 260; elsewhere 262144 x 256 to 8 bits 41 us by pairs and 42.5 by single values, 32768 x
+      // 2048 37 and 38).
       constexpr bool kPairs = G < 1024 && !(MODE == kNormInt8 && VPT == 4);
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
